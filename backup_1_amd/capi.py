@@ -13,6 +13,9 @@ LIB_PATH = os.path.join(_HERE, "libdecx_hip.so")
 
 H2D, D2H, D2D = 1, 2, 3
 CONV_NO_COMPENSATE, CONV_ZERO_COMPENSATE = 0, 1
+F32, F16, BF16 = 0, 1, 2                # element types of the 8-bit operators' wide matrices
+E4M3, E5M2 = 0, 1                       # 8-bit formats
+SCALE_F32, SCALE_E8M0 = 0, 1            # kinds of scale
 
 # every symbol include/decx_hip.h declares; tests check the library exports all of them
 SYMBOLS = [
@@ -25,6 +28,8 @@ SYMBOLS = [
     "decx_hip_conv2_im2col_f32_fused", "decx_hip_conv2_im2col_f16", "decx_hip_conv2_im2col_f16_async", "decx_hip_sgemm_relu", "decx_hip_relu_f32", "decx_hip_relu_f32_async",
     "decx_hip_relu_f32_rec", "decx_hip_relu_f32_backward", "decx_hip_gemm_host_f32", "decx_hip_gemm_host_f16",
     "decx_hip_b_read_extent", "decx_hip_sgemm_plan", "decx_hip_sgemm_plan_split", "decx_hip_hgemm_plan", "decx_hip_hgemm_plan_split", "decx_hip_conv_plan_split", "decx_hip_conv_patch_offsets_fit", "decx_hip_set_splitk_mode", "decx_hip_hgemm_f32acc_noalloc", "decx_hip_release_tmp", "decx_hip_tmp_malloc", "decx_hip_tmp_free",
+    "decx_hip_f8_quantize", "decx_hip_f8_quantize_async", "decx_hip_f8gemm", "decx_hip_f8gemm_async", "decx_hip_rmsnorm_f8",
+    "decx_hip_rmsnorm_f8_async", "decx_hip_rmsnorm_backward", "decx_hip_rmsnorm_backward_async", "decx_hip_rmsnorm_backward_workspace",
 ]
 
 
@@ -87,6 +92,13 @@ def lib():
             "decx_hip_set_splitk_mode": ([I], I),
             "decx_hip_hgemm_f32acc_noalloc": ([P, I, P, I, P, I, P, I, I, I, I, I], I),
         }
+        quantize = [P, I, I, I, I, I, I, I, P, I, P, I, P, I, P, I]
+        f8gemm_args = [P, I, I, P, I, P, I, I, P, I, I, I, P, I, P, I, I, I, I, I]
+        norm = [P, I, P, I, P, ctypes.c_float, I, I, I, P, I, P, P, I, P, I, P, I, I, I]
+        norm_backward = [P, I, P, P, P, I, P, I, I, I, I, P, I, P, P, Z]
+        for name, args in (("f8_quantize", quantize), ("f8gemm", f8gemm_args), ("rmsnorm_f8", norm), ("rmsnorm_backward", norm_backward)):
+            sig["decx_hip_" + name] = sig["decx_hip_" + name + "_async"] = (args, I)
+        sig["decx_hip_rmsnorm_backward_workspace"] = ([I, I], Z)
         for name, (args, res) in sig.items():
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, res
@@ -198,6 +210,31 @@ def conv2_im2col(dsrc, H, W, dpitch, src_row_stride, dfilt, N, kh, kw, filt_stri
     fn = lib().decx_hip_conv2_im2col_f32 if blocking else lib().decx_hip_conv2_im2col_f32_async
     check(fn(dsrc, H, W, dpitch, src_row_stride, dfilt, N, kh, kw, filt_stride, filt_row_stride, ddst, dst_dpitch,
              dst_row_stride, flag))
+
+
+def f8_quantize(dX, ldx, dtype, M, K, block_rows, fmt, scale_type, dQ, ldq, dS, lds, dQt=None, ldqt=0, dSt=None, ldst=0, blocking=True):
+    fn = lib().decx_hip_f8_quantize if blocking else lib().decx_hip_f8_quantize_async
+    check(fn(dX, ldx, dtype, M, K, block_rows, fmt, scale_type, dQ, ldq, dS, lds, dQt, ldqt, dSt, ldst))
+
+
+def f8gemm(dA, lda, fmt_a, dSA, ldsa, dB, ldb, fmt_b, dSB, ldsb, b_block_rows, scale_type, dD, ldd, dtype, M, N, K, dC=None, ldc=0,
+           blocking=True):
+    fn = lib().decx_hip_f8gemm if blocking else lib().decx_hip_f8gemm_async
+    check(fn(dA, lda, fmt_a, dSA, ldsa, dB, ldb, fmt_b, dSB, ldsb, b_block_rows, scale_type, dC, ldc, dD, ldd, dtype, M, N, K))
+
+
+def rmsnorm_f8(dX, ldx, dR, ldr, dW, eps, dtype, M, K, dH, ldh, dRstd, dY, ldy, dQ, ldq, dS, lds, fmt=E4M3, scale_type=SCALE_F32, blocking=True):
+    fn = lib().decx_hip_rmsnorm_f8 if blocking else lib().decx_hip_rmsnorm_f8_async
+    check(fn(dX, ldx, dR, ldr, dW, eps, dtype, M, K, dH, ldh, dRstd, dY, ldy, dQ, ldq, dS, lds, fmt, scale_type))
+
+
+def rmsnorm_backward_workspace(M, K):
+    return lib().decx_hip_rmsnorm_backward_workspace(M, K)
+
+
+def rmsnorm_backward(dH, ldh, dW, dRstd, ddY, lddy, ddR, lddr, dtype, M, K, ddX, lddx, ddW, dWork, work_bytes, blocking=True):
+    fn = lib().decx_hip_rmsnorm_backward if blocking else lib().decx_hip_rmsnorm_backward_async
+    check(fn(dH, ldh, dW, dRstd, ddY, lddy, ddR, lddr, dtype, M, K, ddX, lddx, ddW, dWork, work_bytes))
 
 
 def timer_start():

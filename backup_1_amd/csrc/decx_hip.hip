@@ -58,6 +58,28 @@ int check_gemm_args(const void* A, int lda, const void* B, int ldb, const void* 
     return 0;
 }
 
+int need_library_device() {
+    if (!g_rt.is_init) return need_init();
+    int dev = -1;
+    HIP_TRY(hipGetDevice(&dev));
+    if (dev != g_rt.device)
+        return fail(DECX_HIP_FAIL_ERROR_PARAMS, "the current device is %d, the library was initialised on %d\n", dev, g_rt.device);
+    return 0;
+}
+
+int check_f8_codes(int type, int format, int scale_type) {
+    if (type != DECX_HIP_F32 && type != DECX_HIP_F16 && type != DECX_HIP_BF16) return fail(DECX_HIP_FAIL_ERROR_FLAG, "unknown element type\n");
+    if (format != DECX_HIP_E4M3 && format != DECX_HIP_E5M2) return fail(DECX_HIP_FAIL_ERROR_FLAG, "unknown 8-bit format\n");
+    if (scale_type != DECX_HIP_SCALE_F32 && scale_type != DECX_HIP_SCALE_E8M0) return fail(DECX_HIP_FAIL_ERROR_FLAG, "unknown kind of scale\n");
+    return 0;
+}
+
+int check_element_alignment(const void* p, int type) {
+    if (reinterpret_cast<uintptr_t>(p) & (type == DECX_HIP_F32 ? 3u : 1u))
+        return fail(DECX_HIP_FAIL_ERROR_PARAMS, "matrix off the grid of its elements\n");
+    return 0;
+}
+
 // the fp32 workspace of the fp16 split-K paths: reserved by decx_hip_init for every split the library chooses by itself
 // (at most one 128x128 tile and range per CU, twice that in the atomic mode's tile count), grown only for larger forced
 // splits, kept until the process ends
@@ -695,6 +717,44 @@ int decx_hip_relu_f32_rec(const float* src, float* dst, unsigned char* rec_map, 
 }
 int decx_hip_relu_f32_backward(const float* src, float* dst, const unsigned char* rec_map, size_t n) {
     return finish(relu_enqueue<2>(src, dst, const_cast<unsigned char*>(rec_map), n));
+}
+
+int decx_hip_f8_quantize_async(const void* X, int ldx, int type, int M, int K, int block_rows, int format, int scale_type, uint8_t* Q,
+                               int ldq, void* S, int lds, uint8_t* Qt, int ldqt, void* St, int ldst) {
+    return f8_quantize_enqueue(X, ldx, type, M, K, block_rows, format, scale_type, Q, ldq, S, lds, Qt, ldqt, St, ldst);
+}
+int decx_hip_f8_quantize(const void* X, int ldx, int type, int M, int K, int block_rows, int format, int scale_type, uint8_t* Q, int ldq,
+                         void* S, int lds, uint8_t* Qt, int ldqt, void* St, int ldst) {
+    return finish(f8_quantize_enqueue(X, ldx, type, M, K, block_rows, format, scale_type, Q, ldq, S, lds, Qt, ldqt, St, ldst));
+}
+
+int decx_hip_f8gemm_async(const uint8_t* A, int lda, int format_a, const void* SA, int ldsa, const uint8_t* B, int ldb, int format_b,
+                          const void* SB, int ldsb, int b_block_rows, int scale_type, const void* Cin, int ldc, void* D, int ldd, int type,
+                          int M, int N, int K) {
+    return f8gemm_enqueue(A, lda, format_a, SA, ldsa, B, ldb, format_b, SB, ldsb, b_block_rows, scale_type, Cin, ldc, D, ldd, type, M, N, K);
+}
+int decx_hip_f8gemm(const uint8_t* A, int lda, int format_a, const void* SA, int ldsa, const uint8_t* B, int ldb, int format_b,
+                    const void* SB, int ldsb, int b_block_rows, int scale_type, const void* Cin, int ldc, void* D, int ldd, int type, int M,
+                    int N, int K) {
+    return finish(f8gemm_enqueue(A, lda, format_a, SA, ldsa, B, ldb, format_b, SB, ldsb, b_block_rows, scale_type, Cin, ldc, D, ldd, type, M, N, K));
+}
+
+int decx_hip_rmsnorm_f8_async(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H,
+                              int ldh, float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type) {
+    return rmsnorm_f8_enqueue(X, ldx, R, ldr, W, eps, type, M, K, H, ldh, rstd, Y, ldy, Q, ldq, S, lds, format, scale_type);
+}
+int decx_hip_rmsnorm_f8(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H, int ldh,
+                        float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type) {
+    return finish(rmsnorm_f8_enqueue(X, ldx, R, ldr, W, eps, type, M, K, H, ldh, rstd, Y, ldy, Q, ldq, S, lds, format, scale_type));
+}
+size_t decx_hip_rmsnorm_backward_workspace(int M, int K) { return M > 0 && K > 0 ? rmsnorm_backward_workspace(M, K) : 0; }
+int decx_hip_rmsnorm_backward_async(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR,
+                                    int lddr, int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes) {
+    return rmsnorm_backward_enqueue(H, ldh, W, rstd, dY, lddy, dR, lddr, type, M, K, dX, lddx, dW, work, work_bytes);
+}
+int decx_hip_rmsnorm_backward(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR, int lddr,
+                              int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes) {
+    return finish(rmsnorm_backward_enqueue(H, ldh, W, rstd, dY, lddy, dR, lddr, type, M, K, dX, lddx, dW, work, work_bytes));
 }
 
 int decx_hip_tmp_malloc(void** dptr, size_t bytes) {

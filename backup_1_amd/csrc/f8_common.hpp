@@ -1,0 +1,154 @@
+// What the 8-bit operators share (f8_quantize.hip, f8gemm.hip, rmsnorm.hip): the wide element types and their rounding,
+// the 8-bit codes, the scales of blocks of 128, and loads and stores of 8 consecutive elements at any alignment.
+#pragma once
+#include "tile_common.hpp"
+
+namespace decx_hip {
+
+constexpr int kScaleBlock = 128;      // elements along the contraction that share a scale
+
+// Wide and vector types that may lie at any address: global memory takes such accesses on gfx950 as one instruction, so
+// rows whose pitch is no multiple of 16 bytes need no slower loader of their own.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+
+// ---- wide element types, by the codes of the C ABI (DECX_HIP_F32 / F16 / BF16)
+template <int TYPE> struct Wide;
+template <> struct Wide<0> { typedef float T; };
+template <> struct Wide<1> { typedef _Float16 T; };
+template <> struct Wide<2> { typedef __bf16 T; };
+
+// 8 consecutive elements in fp32 (exact for every type)
+struct Eight {
+    float v[8];
+};
+template <int TYPE>
+__device__ __forceinline__ Eight load8(const typename Wide<TYPE>::T* p) {
+    Eight r;
+    if constexpr (TYPE == 0) {
+        const f32x4 a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.v[e] = a[e], r.v[4 + e] = b[e];
+    } else {
+        typedef typename Wide<TYPE>::T Vec __attribute__((ext_vector_type(8)));
+        const u32x4 raw = *reinterpret_cast<const u32x4_any*>(p);
+        const Vec h = __builtin_bit_cast(Vec, raw);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r.v[e] = (float)h[e];
+    }
+    return r;
+}
+// the first `n` of 8 elements (n <= 8, may be <= 0), the others 0; reads nothing beyond them
+template <int TYPE>
+__device__ __forceinline__ Eight load8_part(const typename Wide<TYPE>::T* p, int n) {
+    if (n >= 8) return load8<TYPE>(p);
+    Eight r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.v[e] = e < n ? (float)p[e] : 0.f;
+    return r;
+}
+// rounds to nearest even, once
+template <int TYPE>
+__device__ __forceinline__ void store8_part(typename Wide<TYPE>::T* p, const Eight& x, int n) {
+    typedef typename Wide<TYPE>::T T;
+    if (n >= 8) {
+        if constexpr (TYPE == 0) {
+            *reinterpret_cast<f32x4_any*>(p) = f32x4{x.v[0], x.v[1], x.v[2], x.v[3]};
+            *reinterpret_cast<f32x4_any*>(p + 4) = f32x4{x.v[4], x.v[5], x.v[6], x.v[7]};
+        } else {
+            typedef T Vec __attribute__((ext_vector_type(8)));
+            Vec h;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = (T)x.v[e];
+            *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, h);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) p[e] = (T)x.v[e];
+}
+
+// ---- 8-bit codes (DECX_HIP_E4M3 / E5M2: the OCP formats, which gfx950 converts to with one rounding to nearest even).
+// The callers' values are within the largest finite one up to the last bit of fp32, which rounds down to it, so no value
+// needs a clamp; a NaN stays a NaN.
+__device__ __forceinline__ uint32_t pack4_f8(float a, float b, float c, float d, int e5m2) {
+    int r = 0;
+    if (e5m2) {
+        r = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, r, false);
+        r = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, r, true);
+    } else {
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, r, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+    }
+    return (uint32_t)r;
+}
+__device__ __forceinline__ u32x2 pack8_f8(const Eight& x, float factor, int e5m2) {
+    return u32x2{pack4_f8(x.v[0] * factor, x.v[1] * factor, x.v[2] * factor, x.v[3] * factor, e5m2),
+                 pack4_f8(x.v[4] * factor, x.v[5] * factor, x.v[6] * factor, x.v[7] * factor, e5m2)};
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, u32x2 codes, int n) {
+    if (n >= 8) {
+        *reinterpret_cast<u32x2_any*>(p) = codes;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) p[e] = (uint8_t)(codes[e >> 2] >> (8 * (e & 3)));
+}
+
+// ---- the scale of a block, from the bits of its largest magnitude.  The maximum is taken over the bit patterns of the
+// magnitudes, which order as the values do with NaN above infinity: a NaN in a block is not lost.
+struct BlockScale {
+    float scale;       // the fp32 scale (the power of two itself for e8m0)
+    float factor;      // what the values are multiplied by before they are rounded to 8 bits
+    uint32_t e8m0;     // its biased exponent
+};
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t eight_magnitude(const Eight& x) {
+    uint32_t m = magnitude_bits(x.v[0]);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+        const uint32_t o = magnitude_bits(x.v[e]);
+        m = m > o ? m : o;
+    }
+    return m;
+}
+constexpr uint32_t kLeastMagnitude = 0x0d800000u;      // 2^-100: blocks of zeros and of smaller values take its scale
+// e4m3's largest value is 1.75 * 2^8, e5m2's 1.75 * 2^15.
+//   fp32: scale = amax / largest, factor = 1 / scale, both correctly rounded: amax * factor is within 2^-22 of the largest.
+//   e8m0: the least 2^e with largest * 2^e >= amax: amax's exponent, one more where its mantissa is beyond 1.75, less 8
+//         (15).  The factor 2^-e is exact, and so is every product with it.  Infinity and NaN give the NaN of e8m0, 255.
+__device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits, int e5m2, int e8m0) {
+    if (amax_bits < kLeastMagnitude) amax_bits = kLeastMagnitude;
+    BlockScale s;
+    if (e8m0) {
+        const uint32_t e = ((amax_bits + 0x1fffffu) >> 23) - (e5m2 ? 15u : 8u);
+        const bool finite = amax_bits < 0x7f800000u;
+        s.e8m0 = finite ? e : 255u;
+        s.scale = finite ? __uint_as_float(e << 23) : __uint_as_float(0x7fc00000u);
+        s.factor = finite ? __uint_as_float((254u - e) << 23) : __uint_as_float(0x7fc00000u);
+    } else {
+        s.scale = __fdiv_rn(__uint_as_float(amax_bits), e5m2 ? 57344.f : 448.f);
+        s.factor = __fdiv_rn(1.f, s.scale);
+        s.e8m0 = 0u;
+    }
+    return s;
+}
+__device__ __forceinline__ void store_scale(void* scales, size_t at, const BlockScale& s, int e8m0) {
+    if (e8m0) static_cast<uint8_t*>(scales)[at] = (uint8_t)s.e8m0;
+    else static_cast<float*>(scales)[at] = s.scale;
+}
+
+// maximum over the 16 lanes of a group (lanes 16g .. 16g + 15), in every lane of it
+__device__ __forceinline__ uint32_t group16_max(uint32_t v) {
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)v, d);
+        v = v > o ? v : o;
+    }
+    return v;
+}
+
+}  // namespace decx_hip

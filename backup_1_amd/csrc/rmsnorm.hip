@@ -1,0 +1,289 @@
+// Root-mean-square norm with the residual's addition, its result as 8-bit codes with a scale for each block of 128 (the
+// left operand of f8gemm.hip) and / or in its own type, and the norm's gradient.
+//
+//   h = round(x + r)      rstd = 1 / sqrt(mean(h^2) + eps)      y = h * rstd * w
+//   n = h * rstd          g = dy * w      dx = rstd * (g - n * mean(g n)) + dr      dw = sum over rows of dy * n
+//
+// Bound: memory, every element read and written once.  A workgroup owns a row at a time and keeps it in registers between
+// the sum over the row and what needs that sum; thread t holds the 8-element chunks t, t + NT, ..., so that 16 consecutive
+// lanes hold a scale block.  Sums are in fp32: at most 32 products in a thread, then a tree over lanes and waves in a fixed
+// order, which gives the same bits on every run.
+#include "runtime.hpp"
+#include "f8_common.hpp"
+
+namespace decx_hip {
+
+// Sum over the workgroup, in every thread.  `part` is used by one call at a time: the callers separate calls by a barrier.
+template <int NT>
+__device__ __forceinline__ float workgroup_sum(float v, float* part) {
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d);
+    if constexpr (NT > kWave) {
+        if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int w = 1; w < NT / kWave; ++w) v += part[w];
+    }
+    return v;
+}
+
+// Consecutive workgroups run on different XCDs; give each XCD a contiguous run of rows, so that the scales of neighbouring
+// rows (4 or 1 bytes each, neighbours in memory) meet in one L2 before they leave it.
+__device__ __forceinline__ int xcd_row(int pid, int rows) {
+    const int xcd = pid % kXcds, local = pid / kXcds, base = rows / kXcds, rem = rows % kXcds;
+    return xcd * base + (xcd < rem ? xcd : rem) + local;
+}
+
+struct RmsNormArgs {
+    const void *X, *R, *W;
+    void *H, *Y;
+    float* rstd;
+    uint8_t* Q;
+    void* S;
+    size_t ldx, ldr, ldh, ldy, ldq, lds;
+    float eps;
+    int M, K, e5m2, e8m0;
+};
+
+template <int TYPE, int NT, int CH>
+__global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
+    typedef typename Wide<TYPE>::T T;
+    __shared__ float part[NT / kWave];
+    const int K = g.K, m = xcd_row((int)blockIdx.x, g.M);
+    const T* x = static_cast<const T*>(g.X) + (size_t)m * g.ldx;
+    Eight h[CH];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+        h[i] = load8_part<TYPE>(x + at, K - k);
+        if (g.R) {
+            const Eight r = load8_part<TYPE>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k);
+            // the sum is what the stream carries on, so it is rounded to its type here and the norm is taken of that
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[i].v[e] = (float)(T)(h[i].v[e] + r.v[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(h[i].v[e], h[i].v[e], sum);
+    }
+    if (g.H) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int k = 8 * ((int)threadIdx.x + i * NT);
+            store8_part<TYPE>(static_cast<T*>(g.H) + (size_t)m * g.ldh + (k < K ? k : 0), h[i], K - k);
+        }
+    }
+    const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(workgroup_sum<NT>(sum, part), (float)K) + g.eps));
+    if (g.rstd && threadIdx.x == 0) g.rstd[m] = rstd;
+    if (!g.Q && !g.Y) return;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+        const Eight w = load8_part<TYPE>(static_cast<const T*>(g.W) + at, K - k);
+        Eight y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y.v[e] = h[i].v[e] * rstd * w.v[e];
+        if (g.Y) store8_part<TYPE>(static_cast<T*>(g.Y) + (size_t)m * g.ldy + at, y, K - k);
+        if (g.Q) {
+            // the codes are rounded from fp32, not from y's own type; elements past K are zeros
+            if (k + 8 > K) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k + e >= K) y.v[e] = 0.f;               // also where rstd is NaN or infinite
+            }
+            const BlockScale s = block_scale(group16_max(eight_magnitude(y)), g.e5m2, g.e8m0);
+            if (k < K) {
+                store_codes(g.Q + (size_t)m * g.ldq + k, pack8_f8(y, s.factor, g.e5m2), K - k);
+                if ((threadIdx.x & 15) == 0) store_scale(g.S, (size_t)(k / kScaleBlock) * g.lds + m, s, g.e8m0);
+            }
+        }
+    }
+}
+
+struct RmsNormBackwardArgs {
+    const void *H, *W, *dY, *dR;
+    const float* rstd;
+    void* dX;
+    float* partial;           // [workgroups][K], nullptr: no dW wanted
+    size_t ldh, lddy, lddr, lddx;
+    int M, K, rows_each;
+};
+
+// Workgroup b owns rows b * rows_each ...: their dx, and their part of dw in a row of `partial`, which the second kernel
+// adds up in row order (no atomics: the same bits on every run).
+template <int TYPE, int NT, int CH>
+__global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackwardArgs g) {
+    typedef typename Wide<TYPE>::T T;
+    __shared__ float part[2][NT / kWave];
+    const int K = g.K, first = (int)blockIdx.x * g.rows_each;
+    const int last = first + g.rows_each < g.M ? first + g.rows_each : g.M;
+    Eight dw[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[i].v[e] = 0.f;
+    for (int m = first; m < last; ++m) {
+        const float rstd = g.rstd[m];
+        Eight n[CH], dn[CH];                                    // n and g
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+            n[i] = load8_part<TYPE>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k);
+            dn[i] = load8_part<TYPE>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k);
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+            const Eight w = load8_part<TYPE>(static_cast<const T*>(g.W) + at, K - k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                n[i].v[e] *= rstd;
+                dw[i].v[e] = __builtin_fmaf(dn[i].v[e], n[i].v[e], dw[i].v[e]);
+                dn[i].v[e] *= w.v[e];
+                sum = __builtin_fmaf(dn[i].v[e], n[i].v[e], sum);
+            }
+        }
+        // two sets of partial sums in turn: a wave may be a row ahead of another, never two (it meets it in between)
+        const float mean = __fdiv_rn(workgroup_sum<NT>(sum, part[m & 1]), (float)K);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+            Eight dx;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dx.v[e] = rstd * __builtin_fmaf(-n[i].v[e], mean, dn[i].v[e]);
+            if (g.dR) {
+                const Eight dr = load8_part<TYPE>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dx.v[e] += dr.v[e];
+            }
+            store8_part<TYPE>(static_cast<T*>(g.dX) + (size_t)m * g.lddx + at, dx, K - k);
+        }
+    }
+    if (!g.partial) return;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int k = 8 * ((int)threadIdx.x + i * NT);
+        store8_part<0>(g.partial + (size_t)blockIdx.x * K + (k < K ? k : 0), dw[i], K - k);
+    }
+}
+
+// dw[k] = sum of `rows` rows of partial.  A workgroup takes 32 columns; its 16 rows of threads add every 16th row each, two
+// columns a thread, and meet in LDS in thread-row order.
+__global__ __launch_bounds__(256) void rmsnorm_dw_kernel(const float* __restrict__ partial, int rows, int K, float* __restrict__ dW) {
+    __shared__ float part[16][33];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int k = (int)blockIdx.x * 32 + 16 * j + c;
+        float v = 0.f;
+        if (k < K)
+            for (int m = r; m < rows; m += 16) v += partial[(size_t)m * K + k];
+        part[r][16 * j + c] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int k = (int)blockIdx.x * 32 + (int)threadIdx.x;
+        float v = part[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) v += part[i][threadIdx.x];
+        if (k < K) dW[k] = v;
+    }
+}
+
+constexpr int kRmsNormMaxK = 32768;       // 1024 threads with 4 chunks each hold a row
+
+// The smallest workgroup that holds a row of K elements with at most 4 chunks a thread, one wave for short rows.
+#define DECX_RMSNORM_SHAPES(K, LAUNCH)       \
+    do {                                     \
+        if ((K) <= 512) LAUNCH(64, 1);       \
+        else if ((K) <= 2048) LAUNCH(256, 1); \
+        else if ((K) <= 4096) LAUNCH(256, 2); \
+        else if ((K) <= 8192) LAUNCH(256, 4); \
+        else if ((K) <= 16384) LAUNCH(512, 4); \
+        else LAUNCH(1024, 4);                \
+    } while (0)
+
+template <int TYPE>
+static int rmsnorm_f8_launch(const RmsNormArgs& g) {
+#define DECX_LAUNCH(NT, CH) hipLaunchKernelGGL((rmsnorm_f8_kernel<TYPE, NT, CH>), dim3((unsigned)g.M), dim3(NT), 0, g_rt.stream, g)
+    DECX_RMSNORM_SHAPES(g.K, DECX_LAUNCH);
+#undef DECX_LAUNCH
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+template <int TYPE>
+static int rmsnorm_backward_launch(const RmsNormBackwardArgs& g, int groups) {
+#define DECX_LAUNCH(NT, CH) hipLaunchKernelGGL((rmsnorm_backward_kernel<TYPE, NT, CH>), dim3((unsigned)groups), dim3(NT), 0, g_rt.stream, g)
+    DECX_RMSNORM_SHAPES(g.K, DECX_LAUNCH);
+#undef DECX_LAUNCH
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H, int ldh,
+                       float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type) {
+    if (int rc = need_library_device()) return rc;
+    if (!X || !W) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "null matrix pointer\n");
+    if (!H && !Y && !Q && !rstd) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "no result wanted\n");
+    if (Q && !S) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "codes without their scales\n");
+    if (M <= 0 || K <= 0) return fail(DECX_HIP_FAIL_DIMS, "Matrix Dims don't match each other");
+    if (K > kRmsNormMaxK) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "the norm takes rows of at most %d elements\n", kRmsNormMaxK);
+    if (int rc = check_f8_codes(type, format, scale_type)) return rc;
+    if (!(eps >= 0.f)) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "eps is negative or no number\n");
+    if (ldx < K || (R && ldr < K) || (H && ldh < K) || (Y && ldy < K) || (Q && (ldq < K || lds < M)))
+        return fail(DECX_HIP_FAIL_ERROR_PARAMS, "leading dimension smaller than the row length\n");
+    for (const void* p : {X, R, W, static_cast<const void*>(H), static_cast<const void*>(Y)})
+        if (int rc = check_element_alignment(p, type)) return rc;
+    if (int rc = check_element_alignment(rstd, DECX_HIP_F32)) return rc;
+    if (Q && scale_type == DECX_HIP_SCALE_F32 && (reinterpret_cast<uintptr_t>(S) & 3u))
+        return fail(DECX_HIP_FAIL_ERROR_PARAMS, "scales off the grid of their type\n");
+    RmsNormArgs g = {};
+    g.X = X, g.R = R, g.W = W, g.H = H, g.Y = Y, g.rstd = rstd, g.Q = Q, g.S = S;
+    g.ldx = (size_t)ldx, g.ldr = (size_t)ldr, g.ldh = (size_t)ldh, g.ldy = (size_t)ldy, g.ldq = (size_t)ldq, g.lds = (size_t)lds;
+    g.eps = eps, g.M = M, g.K = K, g.e5m2 = format == DECX_HIP_E5M2, g.e8m0 = scale_type == DECX_HIP_SCALE_E8M0;
+    if (type == DECX_HIP_F32) return rmsnorm_f8_launch<0>(g);
+    if (type == DECX_HIP_F16) return rmsnorm_f8_launch<1>(g);
+    return rmsnorm_f8_launch<2>(g);
+}
+
+// workgroups of the gradient: two for each compute unit, or one for each row
+static int rmsnorm_backward_groups(int M) {
+    const int most = 2 * (g_rt.compute_units > 0 ? g_rt.compute_units : 256);
+    const int groups = M < most ? M : most;
+    return cdiv(M, cdiv(M, groups));                            // none without rows
+}
+
+size_t rmsnorm_backward_workspace(int M, int K) { return (size_t)rmsnorm_backward_groups(M) * K * sizeof(float); }
+
+int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR, int lddr,
+                             int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes) {
+    if (int rc = need_library_device()) return rc;
+    if (!H || !W || !rstd || !dY || !dX) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "null matrix pointer\n");
+    if (M <= 0 || K <= 0) return fail(DECX_HIP_FAIL_DIMS, "Matrix Dims don't match each other");
+    if (K > kRmsNormMaxK) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "the norm takes rows of at most %d elements\n", kRmsNormMaxK);
+    if (int rc = check_f8_codes(type, DECX_HIP_E4M3, DECX_HIP_SCALE_F32)) return rc;
+    if (ldh < K || lddy < K || (dR && lddr < K) || lddx < K)
+        return fail(DECX_HIP_FAIL_ERROR_PARAMS, "leading dimension smaller than the row length\n");
+    for (const void* p : {H, W, dY, dR, static_cast<const void*>(dX)})
+        if (int rc = check_element_alignment(p, type)) return rc;
+    for (const void* p : {static_cast<const void*>(rstd), static_cast<const void*>(dW)})
+        if (int rc = check_element_alignment(p, DECX_HIP_F32)) return rc;
+    if (dW && (!work || (reinterpret_cast<uintptr_t>(work) & 3u) || work_bytes < rmsnorm_backward_workspace(M, K)))
+        return fail(DECX_HIP_FAIL_ERROR_PARAMS, "the weight's gradient needs a workspace of %zu bytes (decx_hip_rmsnorm_backward_workspace)\n",
+                    rmsnorm_backward_workspace(M, K));
+    const int groups = rmsnorm_backward_groups(M);
+    RmsNormBackwardArgs g = {};
+    g.H = H, g.W = W, g.dY = dY, g.dR = dR, g.rstd = rstd, g.dX = dX, g.partial = dW ? static_cast<float*>(work) : nullptr;
+    g.ldh = (size_t)ldh, g.lddy = (size_t)lddy, g.lddr = (size_t)lddr, g.lddx = (size_t)lddx;
+    g.M = M, g.K = K, g.rows_each = cdiv(M, groups);
+    int rc = type == DECX_HIP_F32 ? rmsnorm_backward_launch<0>(g, groups)
+                                  : type == DECX_HIP_F16 ? rmsnorm_backward_launch<1>(g, groups) : rmsnorm_backward_launch<2>(g, groups);
+    if (rc || !dW) return rc;
+    hipLaunchKernelGGL(rmsnorm_dw_kernel, dim3((unsigned)cdiv(K, 32)), dim3(256), 0, g_rt.stream, g.partial, groups, K, dW);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+}  // namespace decx_hip

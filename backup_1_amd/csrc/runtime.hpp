@@ -71,6 +71,13 @@ struct Batch {
 int check_gemm_args(const void* A, int lda, const void* B, int ldb, const void* Cin, int ldc, const void* D, int ldd, int M,
                     int N, int K, const Batch& batch);
 
+// the 8-bit operators: initialised, and the calling thread's current device is the library's (its stream and kernels are)
+int need_library_device();
+// codes of decx_hip.h for a wide element type, an 8-bit format and a kind of scale
+int check_f8_codes(int type, int format, int scale_type);
+// a matrix must lie on the grid of its own elements (nullptr does)
+int check_element_alignment(const void* p, int type);
+
 // zero-fills the M x N region of a pitched matrix on `stream` (the split-K kernels accumulate into it)
 void enqueue_zero_region(float* D, int ldd, int M, int N, hipStream_t stream);
 
@@ -99,6 +106,16 @@ int hgemm_splitk_static_enqueue(const uint16_t* A, int lda, const uint16_t* B, i
                                 uint16_t* D, int ldd, int M, int N, int K, int splits);
 // looks up the device address of the static workspace for the current device and prepares the kernels that use it
 int hgemm_static_scratch_init(int device);
+int f8_quantize_enqueue(const void* X, int ldx, int type, int M, int K, int block_rows, int format, int scale_type, uint8_t* Q, int ldq,
+                        void* S, int lds, uint8_t* Qt, int ldqt, void* St, int ldst);
+int f8gemm_enqueue(const uint8_t* A, int lda, int format_a, const void* SA, int ldsa, const uint8_t* B, int ldb, int format_b,
+                   const void* SB, int ldsb, int b_block_rows, int scale_type, const void* Cin, int ldc, void* D, int ldd, int type, int M,
+                   int N, int K);
+int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H, int ldh,
+                       float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type);
+size_t rmsnorm_backward_workspace(int M, int K);
+int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR, int lddr,
+                             int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes);
 int hconv_enqueue(const uint16_t* src, int H, int W, int dpitch, size_t src_row_stride, const uint16_t* filt, int N, int kh,
                   int kw, size_t filt_stride, size_t filt_row_stride, uint16_t* dst, int dst_dpitch, size_t dst_row_stride,
                   int flag, const uint16_t* bias, bool relu);

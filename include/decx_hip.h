@@ -242,6 +242,82 @@ int decx_hip_relu_f32_async(const float* src, float* dst, size_t n);
 int decx_hip_relu_f32_rec(const float* src, float* dst, unsigned char* rec_map, size_t n);
 int decx_hip_relu_f32_backward(const float* src, float* dst, const unsigned char* rec_map, size_t n);
 
+/* ---- Products of 8-bit operands, scaled by blocks of 128, and the operators that make such operands: what a layer of a
+ * language model runs on.  The reference has no 8-bit arithmetic; these stand beside decx_hip_hgemm_f32acc and the ReLU
+ * family in the same manner: the same conventions, error codes, library stream, and _async forms.  They take no workspace
+ * of the library and allocate nothing, so any of them may be captured into a graph, and graphs and calls that share no
+ * result (or caller's workspace) may overlap.  The calling thread's current device must be the one decx_hip_init saw.
+ * Matrices may lie at any address that is a multiple of their element's size, with any pitch; D, Q, H, Y and dX are
+ * written within their rows only, and nothing beyond a row's K (N) elements is read.  Sizes are at least 1. */
+
+/* element types of the wide matrices: fp32, IEEE binary16, bfloat16 */
+#define DECX_HIP_F32  0
+#define DECX_HIP_F16  1
+#define DECX_HIP_BF16 2
+/* 8-bit formats (OCP 8-bit floating point): e4m3 holds up to 448 and has no infinity, e5m2 up to 57344 */
+#define DECX_HIP_E4M3 0
+#define DECX_HIP_E5M2 1
+/* scales: fp32, or a power of two 2^(e - 127) as its biased exponent e in 8 bits (255 = NaN).  The matrix instructions
+ * apply the latter themselves: products of such operands are the faster ones. */
+#define DECX_HIP_SCALE_F32  0
+#define DECX_HIP_SCALE_E8M0 1
+
+/* Quantises the M x K matrix X: in blocks of 1 x 128 (block_rows = 1) or 128 x 128 (block_rows = 128) elements, blocks
+ * starting at multiples of 128, the last ones smaller,
+ *   amax = max(|x| over the block, 2^-100)
+ *   fp32 scales: s = amax / largest;  e8m0: s = the least power of two with largest * s >= amax
+ *   Q[m*ldq + k] = x * (1 / s) rounded to the format, nearest even       (1 / s correctly rounded to fp32)
+ * with largest = 448 or 57344.  Scales lie block column by block column: S[kb*lds + m / block_rows], kb = k / 128.
+ * A block that holds NaN has a NaN scale; one that holds an infinity an infinite (fp32) or NaN (e8m0) one, and its value
+ * code * s is NaN everywhere.
+ * Qt, St (nullable, as are Q, S): the same of the transpose, K x M, in blocks along M: Qt[k*ldqt + m], scales
+ * St[mb*ldst + k / block_rows], mb = m / 128 -- for block_rows = 128 the same codes and scales transposed.  One pass over
+ * X makes both.  Q of activations and weights are the operands of the forward product; Qt of the weight (squares) those of
+ * the input's gradient; Qt of activations and of output gradients (rows) those of the weight's gradient. */
+int decx_hip_f8_quantize(const void* X, int ldx, int type, int M, int K, int block_rows, int format, int scale_type, uint8_t* Q, int ldq,
+                         void* S, int lds, uint8_t* Qt, int ldqt, void* St, int ldst);
+int decx_hip_f8_quantize_async(const void* X, int ldx, int type, int M, int K, int block_rows, int format, int scale_type, uint8_t* Q,
+                               int ldq, void* S, int lds, uint8_t* Qt, int ldqt, void* St, int ldst);
+
+/* Product of 8-bit operands with a scale for each block of 128 along K:
+ *   D[m*ldd + n] = Cin[m*ldc + n] + sum over kb of SA[kb*ldsa + m] * SB[kb*ldsb + n / b_block_rows]
+ *                                                  * sum over k in [128 kb, min(128 kb + 128, K)) of A[m*lda + k] * B[n*ldb + k]
+ * A is M x K with a scale for each row and block; B holds one column of the product per row (N x K, as the convolutions'
+ * filter banks), with a scale for each row (b_block_rows = 1) or each 128 rows (128) and block: what decx_hip_f8_quantize
+ * writes.  Each operand has a format of its own, both have scales of one kind.  Cin (nullable, may be D itself with
+ * ldc = ldd) and D have the element type `type`; everything is accumulated in fp32 and rounded to it once.  The 8-bit
+ * matrix instructions add the products of 8 consecutive k with 13 bits below the largest of them: binary16 and bfloat16
+ * results are computed by them, fp32 results by the binary16 instructions on the same codes, which add in full, at half
+ * the rate.  The same bits on every run: work that is split along K is joined in order. */
+int decx_hip_f8gemm(const uint8_t* A, int lda, int format_a, const void* SA, int ldsa, const uint8_t* B, int ldb, int format_b,
+                    const void* SB, int ldsb, int b_block_rows, int scale_type, const void* Cin, int ldc, void* D, int ldd, int type, int M,
+                    int N, int K);
+int decx_hip_f8gemm_async(const uint8_t* A, int lda, int format_a, const void* SA, int ldsa, const uint8_t* B, int ldb, int format_b,
+                          const void* SB, int ldsb, int b_block_rows, int scale_type, const void* Cin, int ldc, void* D, int ldd, int type,
+                          int M, int N, int K);
+
+/* Root-mean-square norm of the rows of X + R (R nullable: of X), K <= 32768:
+ *   h = x + r rounded to `type`;  rstd = 1 / sqrt(mean of h^2 over the row + eps);  y = h * rstd * w
+ * Results, each nullable but not all: H (may be X or R itself, at its pitch), rstd (M floats; what the gradient needs), Y in
+ * `type`, and Q, S: y -- in fp32, not rounded to `type` before -- as decx_hip_f8_quantize gives it with block_rows = 1.
+ * W holds K elements of `type`.  Sums are in fp32. */
+int decx_hip_rmsnorm_f8(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H, int ldh,
+                        float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type);
+int decx_hip_rmsnorm_f8_async(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H,
+                              int ldh, float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type);
+
+/* Its gradient: with n = h * rstd and g = dy * w,
+ *   dx = rstd * (g - n * mean of g n over the row) + dr       (the gradient of X and of R; dR, nullable, is what comes back
+ *                                                              through H itself; dX may be dY, dR or H at its pitch)
+ *   dW[k] = sum over the rows of dy * n                       (K floats; nullable)
+ * dW takes a workspace of the caller of decx_hip_rmsnorm_backward_workspace(M, K) bytes, 4-byte aligned, which need not be
+ * cleared and must not be shared by calls that overlap; the rows' parts are added in order, the same bits on every run. */
+size_t decx_hip_rmsnorm_backward_workspace(int M, int K);
+int decx_hip_rmsnorm_backward(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR, int lddr,
+                              int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes);
+int decx_hip_rmsnorm_backward_async(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR,
+                                    int lddr, int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes);
+
 /* de::release_all_tmp (core/memory_management/Memory_pool.h:23-37: releases the blocks its memory pools hold).  The
  * host-matrix entry points (decx_hip_gemm_host_*, decx_hip_gemm3_host_*) keep their device blocks for the next call, as
  * the reference's device pool does (MemoryPool_D.h); this waits for the device and frees them. */

@@ -1,0 +1,256 @@
+"""decx_hip_rmsnorm_f8 and decx_hip_rmsnorm_backward against 64-bit arithmetic; the gradient also against differences."""
+import numpy as np
+import pytest
+
+import f8_reference as ref
+from backup_1_amd import capi, workloads
+from f8_reference import Pitched
+
+pytestmark = pytest.mark.gpu
+TYPES = (capi.F32, capi.F16, capi.BF16)
+EPS = 1e-5
+# A sum over a row: at most 32 terms in a thread, 6 steps over the lanes, 15 over the waves, a rounding in each product; in
+# steps of 2^-24 of the sum of the magnitudes
+SUM = 60 * 2.0 ** -24
+
+
+def inputs(M, K, kind, seed):
+    x = workloads.normal((M, K), seed).astype(np.float32)
+    x[:, ::13] *= 15.0
+    r = workloads.normal((M, K), seed + 1).astype(np.float32) * 2
+    w = 1 + 0.2 * workloads.normal((K,), seed + 2).astype(np.float32)
+    return [ref.to_type(v, kind) for v in (x, r, w)]
+
+
+def run(x, r, w, kind, fmt=capi.E4M3, scale=capi.SCALE_F32, eps=EPS, want="HsYQ", inplace=None, pitch=0, lead=0):
+    M, K = x.shape
+    st = np.float32 if scale == capi.SCALE_F32 else np.uint8
+    kw = dict(pitch=K + pitch, lead=lead)
+    dx, dw = Pitched(x, **kw), Pitched(w, lead=lead)
+    dr = Pitched(r, **kw) if r is not None else None
+    H = (dx if inplace == "x" else dr if inplace == "r" else Pitched.empty(M, K, x.dtype, **kw)) if "H" in want else None
+    Y = Pitched.empty(M, K, x.dtype, **kw) if "Y" in want else None
+    rstd = Pitched.empty(1, M, np.float32) if "s" in want else None
+    Q = Pitched.empty(M, K, np.uint8, **kw) if "Q" in want else None
+    S = Pitched.empty(-(-K // 128), M, st, pitch=M + pitch, lead=lead) if "Q" in want else None
+    p = lambda b: (b.ptr, b.ld) if b is not None else (None, 0)  # noqa: E731
+    capi.rmsnorm_f8(dx.ptr, dx.ld, *p(dr), dw.ptr, eps, kind, M, K, *p(H), p(rstd)[0], *p(Y), *p(Q), *p(S), fmt, scale)
+    return {n: b.result() if b is not None else None for n, b in (("H", H), ("Y", Y), ("rstd", rstd), ("Q", Q), ("S", S))}
+
+
+def check(x, r, w, kind, got, fmt=capi.E4M3, scale=capi.SCALE_F32, eps=EPS):
+    M, K = x.shape
+    h = x
+    if r is not None:                                            # fp32 holds the sum of two 16-bit values to one rounding
+        h = ref.to_type(ref.from_type(x, kind).astype(np.float32) + ref.from_type(r, kind).astype(np.float32), kind)
+    if got["H"] is not None:
+        assert np.array_equal(got["H"].view(np.uint8), h.view(np.uint8))
+    v = ref.from_type(h, kind)
+    rstd = 1 / np.sqrt((v * v).mean(1) + eps)
+    if got["rstd"] is not None:                                  # half of the sum's error, then division, addition, root, division
+        assert np.all(np.abs(got["rstd"][0] - rstd) <= rstd * (SUM / 2 + 4 * 2.0 ** -24))
+    y = v * rstd[:, None] * ref.from_type(w, kind)
+    off = np.abs(y) * (SUM / 2 + 6 * 2.0 ** -24)                 # and two products
+    if got["Y"] is not None:
+        err = np.abs(ref.from_type(got["Y"], kind) - y)
+        assert np.all(err <= off + np.abs(y) * ref.HALF_STEP[kind] * 1.001 + (2.0 ** -25 if kind == capi.F16 else 0))
+    if got["Q"] is not None:
+        s = ref.scale_values(got["S"]).T                         # [row][block]
+        amax = np.maximum(ref.block_amax(y, 1), 2.0 ** -100)
+        least = amax / ref.LARGEST[fmt]
+        if scale == capi.SCALE_F32:
+            assert np.all(np.abs(s - least) <= least * (SUM / 2 + 8 * 2.0 ** -24))
+        else:                                                    # the least power of two, up to the error of amax at its border
+            assert np.all((s >= least * (1 - 1e-5)) & (s < 2 * least * (1 + 1e-5)))
+        full = ref.spread(s.T, M, K, 1)
+        codes = ref.TABLE[fmt][got["Q"]]
+        # half a step of the grid at the value, or half its smallest step, and the errors of y and of 1 / s
+        half, tiny = (2.0 ** -4, 2.0 ** -10) if fmt == capi.E4M3 else (2.0 ** -3, 2.0 ** -17)
+        assert np.all(np.abs(codes * full - y) <= np.maximum(np.abs(y) * half, tiny * full) * (1 + 1e-5) + off + np.abs(y) * 3 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 100), (1, 4096), (3, 129), (5, 512), (4, 513), (17, 1500), (9, 2048), (9, 2049), (3, 4097), (3, 8192), (2, 8200),
+                                 (2, 16384), (2, 16385), (1, 32768), (300, 384)])
+def test_sizes_and_types(gpu, kind, M, K):
+    x, r, w = inputs(M, K, kind, M + K)
+    check(x, r, w, kind, run(x, r, w, kind))
+    check(x, None, w, kind, run(x, None, w, kind))
+
+
+@pytest.mark.parametrize("fmt", [capi.E4M3, capi.E5M2])
+@pytest.mark.parametrize("scale", [capi.SCALE_F32, capi.SCALE_E8M0])
+def test_formats_and_scales(gpu, fmt, scale):
+    x, r, w = inputs(33, 700, capi.BF16, 4)
+    check(x, r, w, capi.BF16, run(x, r, w, capi.BF16, fmt, scale), fmt, scale)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+def test_pitches_alignment_and_results_left_out(gpu, kind):
+    x, r, w = inputs(20, 333, kind, 6)
+    for want in ("HsYQ", "H", "s", "Y", "Q", "HQ", "sY"):
+        for pitch, lead in ((0, 0), (1, 1), (11, 3), (64, 16)):
+            check(x, r, w, kind, run(x, r, w, kind, want=want, pitch=pitch, lead=lead))
+
+
+def test_sum_written_over_an_input(gpu):
+    x, r, w = inputs(30, 900, capi.F16, 7)
+    for where in ("x", "r"):
+        check(x, r, w, capi.F16, run(x, r, w, capi.F16, inplace=where))
+
+
+def test_rows_of_zeros_and_rows_that_are_not_finite(gpu):
+    x, r, w = inputs(6, 300, capi.F32, 8)
+    x[1] = r[1] = 0
+    x[2, 299], x[4, 5] = np.nan, np.inf
+    got = run(x, r, w, capi.F32)
+    good = [0, 1, 3, 5]
+    check(x[good], r[good], w, capi.F32, {n: (v[:, good] if n in ("rstd", "S") else v[good]) for n, v in got.items()})
+    assert np.isnan(got["rstd"][0, 2]) and got["rstd"][0, 4] == 0
+    assert np.all(np.isnan(got["Y"][2])) and np.isnan(got["Y"][4, 5]) and np.all(np.isnan(got["S"][:, 2]))
+    zero = run(np.zeros((2, 50), np.float32), None, w[:50], capi.F32, eps=0.0)          # no eps: 0 * infinity
+    assert np.all(np.isnan(zero["Y"])) and np.all(np.isinf(zero["rstd"])) and np.all(np.isnan(zero["S"]))
+
+
+def backward(h, w, rstd, dy, dr, kind, want_dw=True, inplace=None, pitch=0, lead=0):
+    M, K = h.shape
+    kw = dict(pitch=K + pitch, lead=lead)
+    dH, dW, dS, dY = Pitched(h, **kw), Pitched(w, lead=lead), Pitched(rstd), Pitched(dy, **kw)
+    dR = Pitched(dr, **kw) if dr is not None else None
+    dX = {"h": dH, "y": dY, "r": dR}[inplace] if inplace else Pitched.empty(M, K, h.dtype, **kw)
+    need = capi.rmsnorm_backward_workspace(M, K)
+    work = Pitched(np.full((1, need), 0xFF, np.uint8))           # NaNs: nothing in it may matter; the guard behind it is checked
+    dw = Pitched.empty(1, K, np.float32, lead=lead) if want_dw else None
+    capi.rmsnorm_backward(dH.ptr, dH.ld, dW.ptr, dS.ptr, dY.ptr, dY.ld, dR.ptr if dR else None, dR.ld if dR else 0, kind, M, K, dX.ptr, dX.ld,
+                          dw.ptr if dw else None, work.ptr if dw else None, need if dw else 0)
+    work.result()
+    return dX.result(), dw.result()[0] if dw else None
+
+
+def gradient64(h, w, rstd, dy, dr):
+    n = h * rstd[:, None]
+    g = dy * w
+    dx = rstd[:, None] * (g - n * (g * n).mean(1, keepdims=True)) + dr
+    size = rstd[:, None] * (np.abs(g) + np.abs(n) * np.abs(g * n).mean(1, keepdims=True))
+    return dx, size, (dy * n).sum(0), np.abs(dy * n).sum(0)
+
+
+def check_backward(h, w, rstd, dy, dr, kind, got, M):
+    dx, dw = got
+    f = lambda a: ref.from_type(a, kind)  # noqa: E731
+    d = f(dr) if dr is not None else np.zeros(h.shape)
+    want, size, want_w, size_w = gradient64(f(h), f(w), rstd.astype(np.float64), f(dy), d)
+    err = np.abs(f(dx) - want)
+    # the row's sum, and at most 8 roundings of one element's way; the addition of dr; the rounding to the type
+    assert np.all(err <= size * (SUM + 8 * 2.0 ** -24) + (size + np.abs(d)) * 2.0 ** -23 + np.abs(want) * ref.HALF_STEP[kind] * 1.001 +
+                  (2.0 ** -25 if kind == capi.F16 else 0))
+    if dw is not None:                                           # in order: a workgroup's rows, every 16th workgroup, the 16
+        assert np.all(np.abs(dw - want_w) <= size_w * (M + 20) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 300), (7, 129), (33, 512), (600, 513), (1100, 200), (50, 1500), (20, 2049), (600, 4097), (3, 8200), (5, 16385),
+                                 (2, 32768)])
+def test_gradient(gpu, kind, M, K):
+    h, dy, w = inputs(M, K, kind, M + 2 * K)
+    dr = ref.to_type(workloads.normal((M, K), 77), kind)
+    rstd = (1 / np.sqrt((ref.from_type(h, kind) ** 2).mean(1) + EPS)).astype(np.float32)
+    check_backward(h, w, rstd, dy, dr, kind, backward(h, w, rstd, dy, dr, kind), M)
+    check_backward(h, w, rstd, dy, None, kind, backward(h, w, rstd, dy, None, kind, want_dw=False), M)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+def test_gradient_in_place_and_any_pitch(gpu, kind):
+    h, dy, w = inputs(40, 333, kind, 9)
+    dr = ref.to_type(workloads.normal((40, 333), 78), kind)
+    rstd = (1 / np.sqrt((ref.from_type(h, kind) ** 2).mean(1) + EPS)).astype(np.float32)
+    plain = backward(h, w, rstd, dy, dr, kind)
+    for where in ("h", "y", "r", None):
+        for pitch, lead in ((0, 0), (3, 1), (51, 16)):
+            got = backward(h, w, rstd, dy, dr, kind, inplace=where, pitch=pitch, lead=lead)
+            assert np.array_equal(got[0].view(np.uint8), plain[0].view(np.uint8)) and np.array_equal(got[1], plain[1])
+
+
+def test_gradient_against_differences(gpu):
+    """Of sum(dy * y + dr * h) by each of some inputs and weights: central differences in 64 bits are exact to 1e-7 here."""
+    M, K = 4, 70
+    x, r, w = [ref.from_type(v, capi.F32) for v in inputs(M, K, capi.F32, 10)]
+    dy, dr = workloads.normal((M, K), 11).astype(np.float32), workloads.normal((M, K), 12).astype(np.float32)
+
+    def loss(h, w):
+        return float((dy * h / np.sqrt((h * h).mean(1, keepdims=True) + EPS) * w).sum() + (dr * h).sum())
+
+    h = (x + r).astype(np.float32).astype(np.float64)
+    rstd = (1 / np.sqrt((h * h).mean(1) + EPS)).astype(np.float32)
+    dx, dw = backward(h.astype(np.float32), w.astype(np.float32), rstd, dy, dr, capi.F32)
+    step = 1e-4
+    for m, k in ((0, 0), (1, 13), (2, 69), (3, 31), (0, 26)):
+        e = np.zeros((M, K))
+        e[m, k] = step
+        assert abs((loss(h + e, w) - loss(h - e, w)) / (2 * step) - dx[m, k]) < 2e-5
+    for k in (0, 13, 69):
+        e = np.zeros(K)
+        e[k] = step
+        assert abs((loss(h, w + e) - loss(h, w - e)) / (2 * step) - dw[k]) < 2e-5
+
+
+def test_same_bits_again(gpu):
+    h, dy, w = inputs(700, 1000, capi.BF16, 13)
+    rstd = (1 / np.sqrt((ref.from_type(h, capi.BF16) ** 2).mean(1) + EPS)).astype(np.float32)
+    a, b = (backward(h, w, rstd, dy, None, capi.BF16) for _ in range(2))
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+    p, q = (run(h, dy, w, capi.BF16) for _ in range(2))
+    assert all(np.array_equal(p[n].view(np.uint8), q[n].view(np.uint8)) for n in p)
+
+
+def test_refusals(gpu):
+    L = capi.lib()
+    d = capi.DeviceBuffer(1 << 18)
+    at = [d.ptr + (i << 14) for i in range(16)]
+    names = ["X", "ldx", "R", "ldr", "W", "eps", "type", "M", "K", "H", "ldh", "rstd", "Y", "ldy", "Q", "ldq", "S", "lds", "format", "scale"]
+    ok = [at[0], 64, at[1], 64, at[2], 1e-5, capi.F32, 32, 64, at[3], 64, at[4], at[5], 64, at[6], 64, at[7], 32, 0, 0]
+
+    def refused(code, **change):
+        assert L.decx_hip_rmsnorm_f8(*[change.get(n, v) for n, v in zip(names, ok)]) == code and capi.last_error().strip(), change
+
+    d.fill(0)
+    assert L.decx_hip_rmsnorm_f8(*ok) == 0
+    refused(0x0d, X=None)
+    refused(0x0d, W=None)
+    refused(0x0d, H=None, Y=None, Q=None, rstd=None)
+    refused(0x0d, S=None)
+    refused(0x03, M=0)
+    refused(0x03, K=0)
+    refused(0x0d, K=32769, ldx=40000, ldr=40000, ldh=40000, ldy=40000, ldq=40000)
+    refused(0x0b, type=9)
+    refused(0x0b, format=2)
+    refused(0x0b, scale=2)
+    refused(0x0d, eps=-1.0)
+    refused(0x0d, eps=float("nan"))
+    for n in ("ldx", "ldr", "ldh", "ldy", "ldq"):
+        refused(0x0d, **{n: 63})
+    refused(0x0d, lds=31)
+    refused(0x0d, H=at[3] + 2)
+    refused(0x0d, rstd=at[4] + 1)
+    refused(0x0d, S=at[7] + 2)
+
+    names = ["H", "ldh", "W", "rstd", "dY", "lddy", "dR", "lddr", "type", "M", "K", "dX", "lddx", "dW", "work", "bytes"]
+    need = capi.rmsnorm_backward_workspace(32, 64)
+    ok = [at[0], 64, at[1], at[2], at[3], 64, at[4], 64, capi.F32, 32, 64, at[5], 64, at[6], at[7], need]
+
+    def refused(code, **change):
+        assert L.decx_hip_rmsnorm_backward(*[change.get(n, v) for n, v in zip(names, ok)]) == code and capi.last_error().strip(), change
+
+    assert need >= 64 * 4 and L.decx_hip_rmsnorm_backward(*ok) == 0
+    for n in ("H", "W", "rstd", "dY", "dX", "work"):
+        refused(0x0d, **{n: None})
+    refused(0x0d, bytes=need - 1)
+    refused(0x0d, work=at[7] + 1)
+    refused(0x03, M=-1)
+    refused(0x03, K=0)
+    refused(0x0d, K=32769, ldh=40000, lddy=40000, lddr=40000, lddx=40000)
+    refused(0x0b, type=-1)
+    for n in ("ldh", "lddy", "lddr", "lddx"):
+        refused(0x0d, **{n: 63})
+    refused(0x0d, dW=at[6] + 2)
+    refused(0x0d, dX=at[5] + 1)
