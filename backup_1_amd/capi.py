@@ -30,6 +30,7 @@ SYMBOLS = [
     "decx_hip_b_read_extent", "decx_hip_sgemm_plan", "decx_hip_sgemm_plan_split", "decx_hip_hgemm_plan", "decx_hip_hgemm_plan_split", "decx_hip_conv_plan_split", "decx_hip_conv_patch_offsets_fit", "decx_hip_set_splitk_mode", "decx_hip_hgemm_f32acc_noalloc", "decx_hip_release_tmp", "decx_hip_tmp_malloc", "decx_hip_tmp_free",
     "decx_hip_f8_quantize", "decx_hip_f8_quantize_async", "decx_hip_f8gemm", "decx_hip_f8gemm_async", "decx_hip_rmsnorm_f8",
     "decx_hip_rmsnorm_f8_async", "decx_hip_rmsnorm_backward", "decx_hip_rmsnorm_backward_async", "decx_hip_rmsnorm_backward_workspace",
+    "decx_hip_set_f8gemm_variant", "decx_hip_f8gemm_plan",
 ]
 
 
@@ -99,6 +100,8 @@ def lib():
         for name, args in (("f8_quantize", quantize), ("f8gemm", f8gemm_args), ("rmsnorm_f8", norm), ("rmsnorm_backward", norm_backward)):
             sig["decx_hip_" + name] = sig["decx_hip_" + name + "_async"] = (args, I)
         sig["decx_hip_rmsnorm_backward_workspace"] = ([I, I], Z)
+        sig["decx_hip_set_f8gemm_variant"] = ([I], I)
+        sig["decx_hip_f8gemm_plan"] = ([I, I, I, I, I, I, ctypes.c_long, ctypes.c_long, I], I)
         for name, (args, res) in sig.items():
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, res

@@ -52,6 +52,7 @@ struct F8GemmArgs {
     int b_shift;            // 7: a scale for each 128 rows of B, 0: for each row
     int type;               // of C and D
     int M, N, K;
+    int variant;            // the kernel to launch (plan_f8gemm, f8gemm.hip)
     int tiles_m, tiles_n, group_m;
 };
 

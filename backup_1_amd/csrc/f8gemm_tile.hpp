@@ -1,0 +1,318 @@
+// Scaled 8-bit product on LDS-DMA tiles: what runs when the result is large enough to fill the chip with tiles.
+//
+// Bound: the matrix pipe.  A K step is one scale block of 128 codes = 128 contiguous bytes of every row of A and of B, so
+// both operands have the same LDS layout: rows of eight 16-byte units, unit q of row r in slot q ^ (r % 8), filled by
+// global_load_lds_dwordx4 with the swizzle on the global side.  A fragment is two ds_read_b128 (units lg and lg + 4 of a
+// row), free of bank conflicts.  The scales of a step's rows and columns travel the same way, 4 bytes of LDS each
+// (global_load_lds_dword, or _ubyte for e8m0), one load a wave, so that the walk waits for nothing but its own stage.
+//
+// Two stages; the walk is unrolled over them, every LDS address is a lane's base plus a constant.  A step is cut into units
+// of two row blocks; a unit's A fragments are read during the unit before it (two sets in turn).  B fragments stay for the
+// whole step.  In the last unit everything of the current stage is in registers: after its first column a barrier (which
+// also says that the next stage has landed), then its refill goes out and the next step's fragments come in, each column of
+// B as soon as its last product is issued.
+//
+// fp32 scales: an instruction's four sums are multiplied into the accumulators two instructions later (`pending`), so that
+// the vector unit never waits for the matrix pipe.
+//
+// Needs 16-byte aligned A and B with pitches in 16s and below 2^24 (32-bit offsets within a tile).
+#pragma once
+#include "f8gemm_common.hpp"
+
+namespace decx_hip {
+
+template <int BM_, int BN_, int WAVES_M_, int WAVES_N_>
+struct F8TileShape {
+    static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, STAGES = 2;
+    static constexpr int NWAVES = WAVES_M * WAVES_N, NT = NWAVES * kWave;
+    static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = WN / 16;
+    static constexpr int UM = 2, UNITS = MI / UM;
+    static constexpr int A_BYTES = BM * kScaleBlock, B_BYTES = BN * kScaleBlock, S_BYTES = (BM + BN) * 4;
+    static constexpr int B_AT = STAGES * A_BYTES, S_AT = B_AT + STAGES * B_BYTES;
+    static constexpr size_t LDS_BYTES = (size_t)S_AT + STAGES * S_BYTES;
+    static constexpr int A_LOADS = BM / 8 / NWAVES, B_LOADS = BN / 8 / NWAVES, LOADS = A_LOADS + B_LOADS + 1;
+    static_assert(UNITS % 2 == 0, "sets of A fragments alternate by unit");
+    static_assert(BM % (8 * NWAVES) == 0 && BN % (8 * NWAVES) == 0, "8 rows a load");
+    static_assert(BM + BN == NT && BM % kWave == 0, "one scale a thread, a wave's all of one operand");
+    static_assert(WN == 64 && 128 % WN == 0, "a wave's columns lie in one 128-row block of B");
+    static_assert(A_BYTES + (MI - 1) * 2048 < 65536 && B_BYTES + (NI - 1) * 2048 < 65536, "16-bit offsets from a lane's base");
+    static_assert(LDS_BYTES <= 160 * 1024, "LDS of a CU");
+};
+
+// 4 bytes (a byte, zero-extended) a lane from global memory to LDS at lds_base + 4 * lane
+template <int TAG, bool BYTE>
+__device__ __forceinline__ void dma_scale(const void* sbase, uint32_t lane_off, uint32_t lds_base) {
+    if constexpr (BYTE)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, %1 ; load %3"
+                     : : "v"(lane_off), "s"(sbase), "s"(lds_base), "n"(TAG) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1 ; load %3"
+                     : : "v"(lane_off), "s"(sbase), "s"(lds_base), "n"(TAG) : "memory", "m0");
+}
+
+template <class S, class F>
+__global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs g) {
+    constexpr int MI = S::MI, NI = S::NI, UM = S::UM, UNITS = S::UNITS, BLK = UM * NI;
+    constexpr bool IN_INSTRUCTION = F::IN_INSTRUCTION, B_PER_ROW = F::B_PER_ROW, EXACT = F::EXACT;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
+    const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)lds_raw;
+    const TileCoord tc = xcd_grouped_tile(blockIdx.x, g.tiles_m, g.tiles_n, g.group_m);
+    const int bm0 = tc.tm * S::BM, bn0 = tc.tn * S::BN;
+    const int tid = threadIdx.x, lane = tid % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int wm0 = (wave / S::WAVES_N) * S::WM, wn0 = (wave % S::WAVES_N) * S::WN;
+    const int lg = lane >> 4, li = lane & 15;
+
+    // ---- DMA sources.  Rows past the end repeat the last one and are never stored.
+    const uint8_t* a_base = g.A + (size_t)bm0 * g.lda;
+    const uint8_t* b_base = g.B + (size_t)bn0 * g.ldb;
+    uint32_t a_off[S::A_LOADS], b_off[S::B_LOADS];
+    const int unit = (lane & 7) ^ (lane >> 3);                  // the unit whose slot of row lane / 8 is lane % 8
+#pragma unroll
+    for (int j = 0; j < S::A_LOADS; ++j) {
+        const int r = (wave * S::A_LOADS + j) * 8 + (lane >> 3), last = g.M - 1 - bm0;
+        a_off[j] = (uint32_t)(r < last ? r : last) * (uint32_t)g.lda + 16u * unit;
+    }
+#pragma unroll
+    for (int j = 0; j < S::B_LOADS; ++j) {
+        const int r = (wave * S::B_LOADS + j) * 8 + (lane >> 3), last = g.N - 1 - bn0;
+        b_off[j] = (uint32_t)(r < last ? r : last) * (uint32_t)g.ldb + 16u * unit;
+    }
+    constexpr uint32_t SCALE_SIZE = F::E8M0 ? 1 : 4;
+    const bool scales_of_a = wave < S::BM / kWave;
+    const uint8_t* s_base = static_cast<const uint8_t*>(scales_of_a ? g.SA : g.SB);
+    const size_t s_step = (scales_of_a ? g.ldsa : g.ldsb) * SCALE_SIZE;
+    uint32_t s_off;
+    {
+        const int m = bm0 + tid, n = bn0 + tid - S::BM;
+        s_off = (uint32_t)(scales_of_a ? (m < g.M ? m : g.M - 1) : (n < g.N ? n : g.N - 1) >> g.b_shift) * SCALE_SIZE;
+    }
+
+    const int full_steps = g.K / kScaleBlock;
+    int steps_fetched = 0;
+    // load J of the next step to fetch; the bases stop at the last whole step, whose loads the last steps repeat
+    auto issue_one = [&](auto stage_tag, auto j_tag) {
+        constexpr int STG = decltype(stage_tag)::value, J = decltype(j_tag)::value;
+        if constexpr (J < S::A_LOADS) {
+            dma_load16_tagged<STG * 64 + J>(a_base, a_off[J], lds_base + (uint32_t)(STG * S::A_BYTES) + (uint32_t)(wave * S::A_LOADS + J) * 1024u);
+        } else if constexpr (J < S::A_LOADS + S::B_LOADS) {
+            constexpr int JB = J - S::A_LOADS;
+            dma_load16_tagged<STG * 64 + J>(b_base, b_off[JB], lds_base + (uint32_t)(S::B_AT + STG * S::B_BYTES) + (uint32_t)(wave * S::B_LOADS + JB) * 1024u);
+        } else {
+            dma_scale<STG * 64 + J, F::E8M0>(s_base, s_off, lds_base + (uint32_t)(S::S_AT + STG * S::S_BYTES) + (uint32_t)wave * 256u);
+            const bool more = ++steps_fetched < full_steps;
+            a_base += more ? kScaleBlock : 0;
+            b_base += more ? kScaleBlock : 0;
+            s_base += more ? s_step : (size_t)0;
+        }
+    };
+
+    f32x4 acc[MI][NI];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // ---- fragments of the current and the next unit, and of B
+    struct Half {
+        u32x4 lo, hi;
+    };
+    Half af[2][UM], bf[NI];
+    uint32_t sa_raw[2][UM], sb_raw[NI];                         // a scale as it lies in LDS, by lane (row li)
+    f32x4 sb_row[NI];                                           // B_PER_ROW: those of columns 4 lg .. 4 lg + 3
+    const uint32_t a_rd = (uint32_t)((wm0 + li) * kScaleBlock + ((lg ^ (li & 7)) << 4));
+    const uint32_t b_rd = (uint32_t)(S::B_AT + (wn0 + li) * kScaleBlock + ((lg ^ (li & 7)) << 4));
+    const uint32_t a_rd4 = a_rd ^ 64u, b_rd4 = b_rd ^ 64u;      // unit lg + 4 instead of lg
+    const uint32_t sa_rd = (uint32_t)(S::S_AT + (wm0 + li) * 4);
+    const uint32_t sb_rd = (uint32_t)(S::S_AT + (S::BM + wn0 + (IN_INSTRUCTION ? li : B_PER_ROW ? 4 * lg : 0)) * 4);
+    auto read_a = [&](auto set_tag, auto stage_tag, auto rb_tag, auto part_tag) {       // part 0, 1: codes, 2: the scale
+        constexpr int SET = decltype(set_tag)::value, STG = decltype(stage_tag)::value, RB = decltype(rb_tag)::value, P = decltype(part_tag)::value;
+        constexpr int OFF = STG * S::A_BYTES + RB * 2048;
+        if constexpr (P == 0) af[SET][RB % UM].lo = *reinterpret_cast<const u32x4*>(lds_raw + a_rd + OFF);
+        else if constexpr (P == 1) af[SET][RB % UM].hi = *reinterpret_cast<const u32x4*>(lds_raw + a_rd4 + OFF);
+        else sa_raw[SET][RB % UM] = *reinterpret_cast<const uint32_t*>(lds_raw + sa_rd + STG * S::S_BYTES + RB * 64);
+    };
+    auto read_b = [&](auto stage_tag, auto ni_tag) {
+        constexpr int STG = decltype(stage_tag)::value, NIX = decltype(ni_tag)::value, OFF = STG * S::B_BYTES + NIX * 2048;
+        bf[NIX].lo = *reinterpret_cast<const u32x4*>(lds_raw + b_rd + OFF);
+        bf[NIX].hi = *reinterpret_cast<const u32x4*>(lds_raw + b_rd4 + OFF);
+        constexpr int S_OFF = STG * S::S_BYTES + NIX * 64;
+        if constexpr (IN_INSTRUCTION) sb_raw[NIX] = *reinterpret_cast<const uint32_t*>(lds_raw + sb_rd + S_OFF);
+        else if constexpr (B_PER_ROW) sb_row[NIX] = *reinterpret_cast<const f32x4*>(lds_raw + sb_rd + S_OFF);
+        else if constexpr (NIX == 0) sb_raw[0] = *reinterpret_cast<const uint32_t*>(lds_raw + sb_rd + STG * S::S_BYTES);
+    };
+    auto scale_value = [&](uint32_t raw) -> float {
+        if constexpr (F::E8M0) return e8m0_value(raw);
+        else return __uint_as_float(raw);
+    };
+
+    // ---- fp32 scales: sums of the last instructions that are not in the accumulators yet
+    constexpr int DELAY = 2, RING = 4;
+    static_assert((UNITS * BLK) % RING == 0, "a step starts at the ring's beginning");
+    struct Pending {
+        f32x4 sum;
+        float s[B_PER_ROW ? 4 : 1];
+    } pending[RING];
+    if constexpr (!IN_INSTRUCTION) {
+#pragma unroll
+        for (int i = 0; i < RING; ++i) {
+            pending[i].sum = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < (B_PER_ROW ? 4 : 1); ++e) pending[i].s[e] = 0.f;
+        }
+    }
+    // MFMA I of unit U works on row block U * UM + row, column ni: column by column, the row order turned on every other
+    // column, so that one operand changes between any two
+    auto settle = [&](auto n_tag) {                             // the sums of instruction N (modulo a step) join the accumulators
+        constexpr int N = (decltype(n_tag)::value + UNITS * BLK) % (UNITS * BLK), U = N / BLK, I = N % BLK;
+        constexpr int R = U * UM + ((I & 1) ^ ((I >> 1) & 1)), C = I >> 1;
+        const Pending& p = pending[N % RING];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[R][C][e] = __builtin_fmaf(p.sum[e], p.s[B_PER_ROW ? e : 0], acc[R][C][e]);
+    };
+    F16Fragment wide_b[NI], wide_a[UM];
+    float row_scale[UM], col_scale = 0.f;
+    auto mfma_one = [&](auto u_tag, auto i_tag) {
+        constexpr int U = decltype(u_tag)::value, I = decltype(i_tag)::value, NIX = I >> 1, ROW = (I & 1) ^ (NIX & 1), SET = U & 1;
+        constexpr int N = U * BLK + I;
+        if constexpr (IN_INSTRUCTION) {
+            acc[U * UM + ROW][NIX] = f8_mfma_scaled<F::FA, F::FB>(f8_fragment(bf[NIX].lo, bf[NIX].hi), f8_fragment(af[SET][ROW].lo, af[SET][ROW].hi),
+                                                                 acc[U * UM + ROW][NIX], (int)sb_raw[NIX], (int)sa_raw[SET][ROW]);
+        } else {
+            if constexpr (I == 0) {
+                if constexpr (U == 0 && !B_PER_ROW) col_scale = scale_value(sb_raw[0]);
+#pragma unroll
+                for (int r = 0; r < UM; ++r) {
+                    row_scale[r] = scale_value(sa_raw[SET][r]) * (B_PER_ROW ? 1.f : col_scale);
+                    if constexpr (EXACT) wide_a[r] = f8_widen<F::FA>(f8_fragment(af[SET][r].lo, af[SET][r].hi));
+                }
+            }
+            if constexpr (EXACT && U == 0 && (I & 1) == 0) wide_b[NIX] = f8_widen<F::FB>(f8_fragment(bf[NIX].lo, bf[NIX].hi));
+            Pending& p = pending[N % RING];
+            if constexpr (EXACT) p.sum = f8_mfma_exact(wide_b[NIX], wide_a[ROW]);
+            else p.sum = f8_mfma<F::FA, F::FB>(f8_fragment(bf[NIX].lo, bf[NIX].hi), f8_fragment(af[SET][ROW].lo, af[SET][ROW].hi), f32x4{0.f, 0.f, 0.f, 0.f});
+            if constexpr (B_PER_ROW) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float s = sb_row[NIX][e];
+                    if constexpr (F::E8M0) s = e8m0_value(__float_as_uint(s));
+                    p.s[e] = row_scale[ROW] * s;
+                }
+            } else {
+                p.s[0] = row_scale[ROW];
+            }
+            settle(std::integral_constant<int, N - DELAY>{});
+        }
+    };
+#define DECX_PIN() __builtin_amdgcn_sched_barrier(0)
+    typedef std::integral_constant<int, 0> I0;
+    typedef std::integral_constant<int, UNITS - 1> Last;
+    // units 0 .. UNITS - 2 of a step: products, and the reads of the next unit's A fragments
+    auto inner_units = [&](auto stage_tag) {
+        static_for<0, UNITS - 1>([&](auto u_tag) {
+            constexpr int U = decltype(u_tag)::value;
+            typedef std::integral_constant<int, (U + 1) & 1> NextSet;
+            static_for<0, BLK>([&](auto i_tag) {
+                constexpr int I = decltype(i_tag)::value;
+                static_assert(BLK >= 3 * UM, "a read a slot");
+                if constexpr (I < 3 * UM)
+                    read_a(NextSet{}, stage_tag, std::integral_constant<int, (U + 1) * UM + I / 3>{}, std::integral_constant<int, I % 3>{});
+                mfma_one(u_tag, i_tag);
+                DECX_PIN();
+            });
+        });
+    };
+    auto k_step = [&](auto stage_tag) {
+        constexpr int STG = decltype(stage_tag)::value;
+        typedef std::integral_constant<int, 1 - STG> Next;
+        inner_units(stage_tag);
+        mfma_one(Last{}, I0{});
+        DECX_PIN();
+        mfma_one(Last{}, std::integral_constant<int, 1>{});
+        DECX_PIN();
+        wait_dma_then_barrier<0>();
+        DECX_PIN();
+        constexpr int SLOTS = BLK - 2;
+        static_for<0, SLOTS>([&](auto s_tag) {
+            constexpr int I = decltype(s_tag)::value;
+            // the next step's first products need column 0 of B and the first row blocks of A: those first
+            if constexpr (I % 2 == 0) read_b(Next{}, std::integral_constant<int, I / 2>{});
+            static_assert(SLOTS >= UM * 3 / 2, "the first unit's A fragments come in at two reads a slot");
+            if constexpr (I < (3 * UM + 1) / 2) {
+                static_for<2 * I, (2 * I + 2 < 3 * UM ? 2 * I + 2 : 3 * UM)>([&](auto r_tag) {
+                    constexpr int R = decltype(r_tag)::value;
+                    read_a(I0{}, Next{}, std::integral_constant<int, R / 3>{}, std::integral_constant<int, R % 3>{});
+                });
+            }
+            static_for<(I * S::LOADS) / SLOTS, ((I + 1) * S::LOADS) / SLOTS>([&](auto j_tag) { issue_one(stage_tag, j_tag); });
+            mfma_one(Last{}, std::integral_constant<int, I + 2>{});
+            DECX_PIN();
+        });
+        read_b(Next{}, std::integral_constant<int, NI - 1>{});
+        DECX_PIN();
+    };
+    auto read_first = [&](auto stage_tag) {
+        static_for<0, 3 * UM>([&](auto r) {
+            constexpr int R = decltype(r)::value;
+            read_a(I0{}, stage_tag, std::integral_constant<int, R / 3>{}, std::integral_constant<int, R % 3>{});
+        });
+        static_for<0, NI>([&](auto ni) { read_b(stage_tag, ni); });
+    };
+
+    if (full_steps > 0) {
+        // an odd number of steps starts in stage 1, so that whole passes over the two stages follow
+        const bool odd = full_steps & 1;
+        typedef std::integral_constant<int, 1> I1;
+        if (odd) {
+            static_for<0, S::LOADS>([&](auto j) { issue_one(I1{}, j); });
+            static_for<0, S::LOADS>([&](auto j) { issue_one(I0{}, j); });
+            wait_dma_then_barrier<S::LOADS>();
+            read_first(I1{});
+            DECX_PIN();
+            k_step(I1{});
+        } else {
+            static_for<0, S::LOADS>([&](auto j) { issue_one(I0{}, j); });
+            static_for<0, S::LOADS>([&](auto j) { issue_one(I1{}, j); });
+            wait_dma_then_barrier<S::LOADS>();
+            read_first(I0{});
+            DECX_PIN();
+        }
+        for (int t = full_steps >> 1; t > 0; --t) {
+            k_step(I0{});
+            k_step(I1{});
+        }
+    }
+    wait_dma_then_barrier<0>();                                 // the last, redundant loads have landed, nobody reads LDS any more
+    if (full_steps * kScaleBlock < g.K) {
+        // ---- the ragged last block, through registers into stage 0, zeros past K
+        const int k0 = full_steps * kScaleBlock;
+        auto fill = [&](const uint8_t* base, size_t pitch, int rows, int last, int at) {
+            for (int id = tid; id < rows * 8; id += S::NT) {
+                const int r = id >> 3, q = id & 7;
+                const u32x4 v = f8_unit_part(base + (size_t)(r < last ? r : last) * pitch + k0 + 16 * q, g.K - k0 - 16 * q);
+                *reinterpret_cast<u32x4*>(lds_raw + at + r * kScaleBlock + ((q ^ (r & 7)) << 4)) = v;
+            }
+        };
+        fill(g.A + (size_t)bm0 * g.lda, g.lda, S::BM, g.M - 1 - bm0, 0);
+        fill(g.B + (size_t)bn0 * g.ldb, g.ldb, S::BN, g.N - 1 - bn0, S::B_AT);
+        {
+            const void* scales = scales_of_a ? g.SA : g.SB;
+            const uint8_t* at = static_cast<const uint8_t*>(scales) + (size_t)full_steps * s_step + s_off;
+            *reinterpret_cast<uint32_t*>(lds_raw + S::S_AT + tid * 4) = F::E8M0 ? (uint32_t)*at : *reinterpret_cast<const uint32_t*>(at);
+        }
+        __syncthreads();
+        read_first(I0{});
+        inner_units(I0{});
+        static_for<0, BLK>([&](auto i) { mfma_one(Last{}, i); });
+    }
+    if constexpr (!IN_INSTRUCTION)
+        static_for<0, DELAY>([&](auto d) { settle(std::integral_constant<int, UNITS * BLK - DELAY + decltype(d)::value>{}); });
+
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < NI; ++ni) f8_store_result(g, bm0 + wm0 + 16 * mi + li, bn0 + wn0 + 16 * ni + 4 * lg, acc[mi][ni]);
+#undef DECX_PIN
+}
+
+}  // namespace decx_hip

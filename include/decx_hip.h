@@ -296,6 +296,12 @@ int decx_hip_f8gemm_async(const uint8_t* A, int lda, int format_a, const void* S
                           const void* SB, int ldsb, int b_block_rows, int scale_type, const void* Cin, int ldc, void* D, int ldd, int type,
                           int M, int N, int K);
 
+/* As decx_hip_set_hgemm_variant and decx_hip_hgemm_plan: forces a kernel where it can take the operands (numbers in
+ * backup_1_amd/csrc/f8gemm.hip; 0 = automatic; returns the previous value), and, host-only, the kernel that
+ * decx_hip_f8gemm takes (-1 on bad sizes; aligned = 0: A or B off the 16-byte grid). */
+int decx_hip_set_f8gemm_variant(int variant);
+int decx_hip_f8gemm_plan(int M, int N, int K, int type, int scale_type, int b_block_rows, long lda, long ldb, int aligned);
+
 /* Root-mean-square norm of the rows of X + R (R nullable: of X), K <= 32768:
  *   h = x + r rounded to `type`;  rstd = 1 / sqrt(mean of h^2 over the row + eps);  y = h * rstd * w
  * Results, each nullable but not all: H (may be X or R itself, at its pitch), rstd (M floats; what the gradient needs), Y in
