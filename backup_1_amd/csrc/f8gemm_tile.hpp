@@ -15,7 +15,8 @@
 // fp32 scales: an instruction's four sums are multiplied into the accumulators two instructions later (`pending`), so that
 // the vector unit never waits for the matrix pipe.
 //
-// Needs 16-byte aligned A and B with pitches in 16s and below 2^24 (32-bit offsets within a tile).
+// Needs 16-byte aligned A and B with pitches in 16s and below 2^24 (32-bit offsets within a tile).  Of a row's last 16-byte
+// unit the bytes past K are read too, and dropped: they lie in the same aligned 16 bytes as one of the row's codes.
 #pragma once
 #include "f8gemm_common.hpp"
 
@@ -88,9 +89,18 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
         s_off = (uint32_t)(scales_of_a ? (m < g.M ? m : g.M - 1) : (n < g.N ? n : g.N - 1) >> g.b_shift) * SCALE_SIZE;
     }
 
-    const int full_steps = g.K / kScaleBlock;
-    int steps_fetched = 0;
-    // load J of the next step to fetch; the bases stop at the last whole step, whose loads the last steps repeat
+    // The walk begins with the last block of K, the only one that may be ragged, and goes on with blocks 0, 1, ...  Its loads
+    // fetch the 16-byte units that hold at least one code of the row (the lanes of the other units fetch the block's first
+    // unit again), and its codes past K are zeroed in registers.
+    const int others = (g.K - 1) / kScaleBlock, codes_first = g.K - others * kScaleBlock;
+    const uint32_t unit_back = 16 * unit >= codes_first ? 16u * unit : 0u;
+#pragma unroll
+    for (int j = 0; j < S::A_LOADS; ++j) a_off[j] -= unit_back;
+#pragma unroll
+    for (int j = 0; j < S::B_LOADS; ++j) b_off[j] -= unit_back;
+    a_base += (size_t)others * kScaleBlock, b_base += (size_t)others * kScaleBlock, s_base += (size_t)others * s_step;
+    int fetches_left = others;
+    // load J of the next step to fetch; the last step's loads are repeated for as long as the walk goes on
     auto issue_one = [&](auto stage_tag, auto j_tag) {
         constexpr int STG = decltype(stage_tag)::value, J = decltype(j_tag)::value;
         if constexpr (J < S::A_LOADS) {
@@ -100,7 +110,7 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
             dma_load16_tagged<STG * 64 + J>(b_base, b_off[JB], lds_base + (uint32_t)(S::B_AT + STG * S::B_BYTES) + (uint32_t)(wave * S::B_LOADS + JB) * 1024u);
         } else {
             dma_scale<STG * 64 + J, F::E8M0>(s_base, s_off, lds_base + (uint32_t)(S::S_AT + STG * S::S_BYTES) + (uint32_t)wave * 256u);
-            const bool more = ++steps_fetched < full_steps;
+            const bool more = --fetches_left > 0;
             a_base += more ? kScaleBlock : 0;
             b_base += more ? kScaleBlock : 0;
             s_base += more ? s_step : (size_t)0;
@@ -120,11 +130,14 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
     Half af[2][UM], bf[NI];
     uint32_t sa_raw[2][UM], sb_raw[NI];                         // a scale as it lies in LDS, by lane (row li)
     f32x4 sb_row[NI];                                           // B_PER_ROW: those of columns 4 lg .. 4 lg + 3
-    const uint32_t a_rd = (uint32_t)((wm0 + li) * kScaleBlock + ((lg ^ (li & 7)) << 4));
-    const uint32_t b_rd = (uint32_t)(S::B_AT + (wn0 + li) * kScaleBlock + ((lg ^ (li & 7)) << 4));
-    const uint32_t a_rd4 = a_rd ^ 64u, b_rd4 = b_rd ^ 64u;      // unit lg + 4 instead of lg
-    const uint32_t sa_rd = (uint32_t)(S::S_AT + (wm0 + li) * 4);
-    const uint32_t sb_rd = (uint32_t)(S::S_AT + (S::BM + wn0 + (IN_INSTRUCTION ? li : B_PER_ROW ? 4 * lg : 0)) * 4);
+    // Every read is one of six lane bases plus a constant of the instruction.  The bases are hidden from the compiler, which
+    // would otherwise fold parts of them into constants beyond the instruction's 16 bits, a register for each.
+    uint32_t a_rd = (uint32_t)((wm0 + li) * kScaleBlock + ((lg ^ (li & 7)) << 4));
+    uint32_t b_rd = (uint32_t)(S::B_AT + (wn0 + li) * kScaleBlock + ((lg ^ (li & 7)) << 4));
+    uint32_t a_rd4 = a_rd ^ 64u, b_rd4 = b_rd ^ 64u;            // unit lg + 4 instead of lg
+    uint32_t sa_rd = (uint32_t)(S::S_AT + (wm0 + li) * 4);
+    uint32_t sb_rd = (uint32_t)(S::S_AT + (S::BM + wn0 + (IN_INSTRUCTION ? li : B_PER_ROW ? 4 * lg : 0)) * 4);
+    asm volatile("" : "+v"(a_rd), "+v"(a_rd4), "+v"(b_rd), "+v"(b_rd4), "+v"(sa_rd), "+v"(sb_rd));
     auto read_a = [&](auto set_tag, auto stage_tag, auto rb_tag, auto part_tag) {       // part 0, 1: codes, 2: the scale
         constexpr int SET = decltype(set_tag)::value, STG = decltype(stage_tag)::value, RB = decltype(rb_tag)::value, P = decltype(part_tag)::value;
         constexpr int OFF = STG * S::A_BYTES + RB * 2048;
@@ -207,25 +220,46 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
 #define DECX_PIN() __builtin_amdgcn_sched_barrier(0)
     typedef std::integral_constant<int, 0> I0;
     typedef std::integral_constant<int, UNITS - 1> Last;
+    // zeros past K in a lane's fragments: its units start at codes 16 lg and 16 lg + 64 of the block
+    auto unit_mask = [&](int first) {
+        u32x4 m;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int n = codes_first - first - 4 * w;                // codes of this word that exist
+            m[w] = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+        }
+        return m;
+    };
     // units 0 .. UNITS - 2 of a step: products, and the reads of the next unit's A fragments
-    auto inner_units = [&](auto stage_tag) {
+    auto inner_units = [&](auto stage_tag, auto ragged_tag, u32x4 keep_lo, u32x4 keep_hi) {
         static_for<0, UNITS - 1>([&](auto u_tag) {
-            constexpr int U = decltype(u_tag)::value;
-            typedef std::integral_constant<int, (U + 1) & 1> NextSet;
+            constexpr int U = decltype(u_tag)::value, SET = (U + 1) & 1;
             static_for<0, BLK>([&](auto i_tag) {
                 constexpr int I = decltype(i_tag)::value;
                 static_assert(BLK >= 3 * UM, "a read a slot");
                 if constexpr (I < 3 * UM)
-                    read_a(NextSet{}, stage_tag, std::integral_constant<int, (U + 1) * UM + I / 3>{}, std::integral_constant<int, I % 3>{});
+                    read_a(std::integral_constant<int, SET>{}, stage_tag, std::integral_constant<int, (U + 1) * UM + I / 3>{}, std::integral_constant<int, I % 3>{});
                 mfma_one(u_tag, i_tag);
                 DECX_PIN();
             });
+            if constexpr (decltype(ragged_tag)::value) {
+#pragma unroll
+                for (int r = 0; r < UM; ++r) af[SET][r].lo &= keep_lo, af[SET][r].hi &= keep_hi;
+            }
         });
     };
-    auto k_step = [&](auto stage_tag) {
+    auto k_step = [&](auto stage_tag, auto ragged_tag) {
         constexpr int STG = decltype(stage_tag)::value;
         typedef std::integral_constant<int, 1 - STG> Next;
-        inner_units(stage_tag);
+        u32x4 keep_lo, keep_hi;
+        if constexpr (decltype(ragged_tag)::value) {
+            keep_lo = unit_mask(16 * lg), keep_hi = unit_mask(16 * lg + 64);
+#pragma unroll
+            for (int r = 0; r < UM; ++r) af[0][r].lo &= keep_lo, af[0][r].hi &= keep_hi;
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) bf[ni].lo &= keep_lo, bf[ni].hi &= keep_hi;
+        }
+        inner_units(stage_tag, ragged_tag, keep_lo, keep_hi);
         mfma_one(Last{}, I0{});
         DECX_PIN();
         mfma_one(Last{}, std::integral_constant<int, 1>{});
@@ -259,52 +293,28 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
         static_for<0, NI>([&](auto ni) { read_b(stage_tag, ni); });
     };
 
-    if (full_steps > 0) {
-        // an odd number of steps starts in stage 1, so that whole passes over the two stages follow
-        const bool odd = full_steps & 1;
-        typedef std::integral_constant<int, 1> I1;
-        if (odd) {
-            static_for<0, S::LOADS>([&](auto j) { issue_one(I1{}, j); });
-            static_for<0, S::LOADS>([&](auto j) { issue_one(I0{}, j); });
-            wait_dma_then_barrier<S::LOADS>();
-            read_first(I1{});
-            DECX_PIN();
-            k_step(I1{});
-        } else {
-            static_for<0, S::LOADS>([&](auto j) { issue_one(I0{}, j); });
-            static_for<0, S::LOADS>([&](auto j) { issue_one(I1{}, j); });
-            wait_dma_then_barrier<S::LOADS>();
-            read_first(I0{});
-            DECX_PIN();
-        }
-        for (int t = full_steps >> 1; t > 0; --t) {
-            k_step(I0{});
-            k_step(I1{});
-        }
+    typedef std::integral_constant<int, 1> I1;
+    static_for<0, S::LOADS>([&](auto j) { issue_one(I1{}, j); });
+    if (others > 0) {
+        a_base = g.A + (size_t)bm0 * g.lda, b_base = g.B + (size_t)bn0 * g.ldb;
+        s_base = static_cast<const uint8_t*>(scales_of_a ? g.SA : g.SB);
+        fetches_left = others;
+#pragma unroll
+        for (int j = 0; j < S::A_LOADS; ++j) a_off[j] += unit_back;
+#pragma unroll
+        for (int j = 0; j < S::B_LOADS; ++j) b_off[j] += unit_back;
     }
-    wait_dma_then_barrier<0>();                                 // the last, redundant loads have landed, nobody reads LDS any more
-    if (full_steps * kScaleBlock < g.K) {
-        // ---- the ragged last block, through registers into stage 0, zeros past K
-        const int k0 = full_steps * kScaleBlock;
-        auto fill = [&](const uint8_t* base, size_t pitch, int rows, int last, int at) {
-            for (int id = tid; id < rows * 8; id += S::NT) {
-                const int r = id >> 3, q = id & 7;
-                const u32x4 v = f8_unit_part(base + (size_t)(r < last ? r : last) * pitch + k0 + 16 * q, g.K - k0 - 16 * q);
-                *reinterpret_cast<u32x4*>(lds_raw + at + r * kScaleBlock + ((q ^ (r & 7)) << 4)) = v;
-            }
-        };
-        fill(g.A + (size_t)bm0 * g.lda, g.lda, S::BM, g.M - 1 - bm0, 0);
-        fill(g.B + (size_t)bn0 * g.ldb, g.ldb, S::BN, g.N - 1 - bn0, S::B_AT);
-        {
-            const void* scales = scales_of_a ? g.SA : g.SB;
-            const uint8_t* at = static_cast<const uint8_t*>(scales) + (size_t)full_steps * s_step + s_off;
-            *reinterpret_cast<uint32_t*>(lds_raw + S::S_AT + tid * 4) = F::E8M0 ? (uint32_t)*at : *reinterpret_cast<const uint32_t*>(at);
-        }
-        __syncthreads();
-        read_first(I0{});
-        inner_units(I0{});
-        static_for<0, BLK>([&](auto i) { mfma_one(Last{}, i); });
+    static_for<0, S::LOADS>([&](auto j) { issue_one(I0{}, j); });
+    wait_dma_then_barrier<S::LOADS>();
+    read_first(I1{});
+    DECX_PIN();
+    k_step(I1{}, std::true_type{});
+    for (int t = others >> 1; t > 0; --t) {
+        k_step(I0{}, std::false_type{});
+        k_step(I1{}, std::false_type{});
     }
+    if (others & 1) k_step(I0{}, std::false_type{});
+    wait_dma_then_barrier<0>();                                 // the redundant loads have landed before the workgroup gives up its LDS
     if constexpr (!IN_INSTRUCTION)
         static_for<0, DELAY>([&](auto d) { settle(std::integral_constant<int, UNITS * BLK - DELAY + decltype(d)::value>{}); });
 

@@ -248,7 +248,8 @@ int decx_hip_relu_f32_backward(const float* src, float* dst, const unsigned char
  * of the library and allocate nothing, so any of them may be captured into a graph, and graphs and calls that share no
  * result (or caller's workspace) may overlap.  The calling thread's current device must be the one decx_hip_init saw.
  * Matrices may lie at any address that is a multiple of their element's size, with any pitch; D, Q, H, Y and dX are
- * written within their rows only, and nothing beyond a row's K (N) elements is read.  Sizes are at least 1. */
+ * written within their rows only; of what lies beyond a row's K (N) elements at most the rest of the aligned 16 bytes that
+ * hold the last one is read, and not used.  Sizes are at least 1. */
 
 /* element types of the wide matrices: fp32, IEEE binary16, bfloat16 */
 #define DECX_HIP_F32  0
