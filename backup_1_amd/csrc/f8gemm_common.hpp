@@ -146,4 +146,29 @@ __device__ __forceinline__ void f8_store_result(const F8GemmArgs& g, int m, int 
         f8_store4(static_cast<__bf16*>(g.D) + d, g.C ? static_cast<const __bf16*>(g.C) + c : nullptr, v, left);
 }
 
+// columns n .. n + 3 of row m of C, as far as they exist, on top of v (16-bit results)
+template <class T>
+__device__ __forceinline__ f32x4 f8_add_c(const F8GemmArgs& g, int m, int n, f32x4 v) {
+    if (m >= g.M || n >= g.N) return v;
+    const T* c = static_cast<const T*>(g.C) + (size_t)m * g.ldc + n;
+    if (n + 4 <= g.N) {
+        typedef T Four __attribute__((ext_vector_type(4)));
+        typedef T FourAny __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        const Four o = *reinterpret_cast<const FourAny*>(c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += (float)o[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < g.N) v[e] += (float)c[e];
+    }
+    return v;
+}
+template <class T>
+__device__ __forceinline__ u32x2 f8_round4(f32x4 v) {
+    typedef T Four __attribute__((ext_vector_type(4)));
+    const Four r = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    return __builtin_bit_cast(u32x2, r);
+}
+
 }  // namespace decx_hip

@@ -318,10 +318,57 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
     if constexpr (!IN_INSTRUCTION)
         static_for<0, DELAY>([&](auto d) { settle(std::integral_constant<int, UNITS * BLK - DELAY + decltype(d)::value>{}); });
 
+    // ---- epilogue.  fp32 results leave as they lie in the accumulators, 16 bytes a lane (through LDS in 256-byte rows: 2 %
+    // slower at 8192^3).  16-bit ones, 8 bytes a lane there, go through LDS (the operands' stages are free) in rows of 16-byte
+    // pieces XOR-swizzled by the row, and leave as whole 128-byte lines (8192^3: 431 -> 400 us).  The wave reads back what it
+    // wrote itself, in order: no barrier.
+    const int m_wave = bm0 + wm0, n_wave = bn0 + wn0;
+    if constexpr (EXACT) {                                      // fp32 results, and only those
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
+        for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
-        for (int ni = 0; ni < NI; ++ni) f8_store_result(g, bm0 + wm0 + 16 * mi + li, bn0 + wn0 + 16 * ni + 4 * lg, acc[mi][ni]);
+            for (int ni = 0; ni < NI; ++ni) f8_store_result(g, m_wave + 16 * mi + li, n_wave + 16 * ni + 4 * lg, acc[mi][ni]);
+    } else {
+        constexpr int ROW_BYTES = S::WN * 2, PIECES = ROW_BYTES / 16, ROWS_PER_PASS = kWave / PIECES;
+        static_assert(PIECES == 8 && (size_t)S::NWAVES * S::WM * ROW_BYTES <= (size_t)S::S_AT, "every wave's piece fits the stages");
+        unsigned char* park = lds_raw + (size_t)wave * (S::WM * ROW_BYTES);
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+                const int row = 16 * mi + li, col = 16 * ni + 4 * lg;
+                f32x4 v = acc[mi][ni];
+                u32x2 r;
+                if (g.type == DECX_HIP_F16) {
+                    if (g.C) v = f8_add_c<_Float16>(g, m_wave + row, n_wave + col, v);
+                    r = f8_round4<_Float16>(v);
+                } else {
+                    if (g.C) v = f8_add_c<__bf16>(g, m_wave + row, n_wave + col, v);
+                    r = f8_round4<__bf16>(v);
+                }
+                *reinterpret_cast<u32x2*>(park + row * ROW_BYTES + (((col >> 3) ^ (row & 7)) << 4) + ((lg & 1) << 3)) = r;
+            }
+        uint16_t* const d = static_cast<uint16_t*>(g.D);
+        const bool whole = bm0 + S::BM <= g.M && bn0 + S::BN <= g.N && ((reinterpret_cast<uintptr_t>(d) | (g.ldd * 2)) & 15) == 0;
+#pragma unroll 4
+        for (int pass = 0; pass < S::WM / ROWS_PER_PASS; ++pass) {
+            const int row = pass * ROWS_PER_PASS + lane / PIECES, piece = lane % PIECES;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(park + row * ROW_BYTES + ((piece ^ (row & 7)) << 4));
+            const int m = m_wave + row, n = n_wave + piece * 8;
+            uint16_t* to = d + (size_t)m * g.ldd + n;
+            if (whole) {
+                __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(to));       // not read by this launch
+            } else if (m < g.M && n < g.N) {
+                if (n + 8 <= g.N) {
+                    *reinterpret_cast<u32x4_any*>(to) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e < g.N) to[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+                }
+            }
+        }
+    }
 #undef DECX_PIN
 }
 
