@@ -83,7 +83,7 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
         const Eight w = load8_part<TYPE>(static_cast<const T*>(g.W) + at, K - k);
         Eight y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y.v[e] = h[i].v[e] * rstd * w.v[e];
+        for (int e = 0; e < 8; ++e) y.v[e] = TYPE == 0 ? h[i].v[e] * rstd * w.v[e] : h[i].v[e] * w.v[e] * rstd;     // 16-bit h * w is exact
         if (g.Y) store8_part<TYPE>(static_cast<T*>(g.Y) + (size_t)m * g.ldy + at, y, K - k);
         if (g.Q) {
             // the codes are rounded from fp32, not from y's own type; elements past K are zeros
@@ -123,20 +123,35 @@ __global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackw
     for (int i = 0; i < CH; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[i].v[e] = 0.f;
+    // the next row's loads are in flight while a row waits for its sum
+    struct Row {
+        RawEight<TYPE> h[CH], dy[CH], dr[CH];
+        float rstd;
+    };
+    auto load_row = [&](Row& r, int m) {
+        r.rstd = g.rstd[m];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+            r.h[i] = load_raw8_part<TYPE>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k);
+            r.dy[i] = load_raw8_part<TYPE>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k);
+            if (g.dR) r.dr[i] = load_raw8_part<TYPE>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
+        }
+    };
+    Row next;
+    load_row(next, first);
     for (int m = first; m < last; ++m) {
-        const float rstd = g.rstd[m];
+        const Row row = next;
+        if (m + 1 < last) load_row(next, m + 1);
+        const float rstd = row.rstd;
         Eight n[CH], dn[CH];                                    // n and g
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            n[i] = load8_part<TYPE>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k);
-            dn[i] = load8_part<TYPE>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k);
-        }
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
             const Eight w = load8_part<TYPE>(static_cast<const T*>(g.W) + at, K - k);
+            n[i] = widen8<TYPE>(row.h[i]);
+            dn[i] = widen8<TYPE>(row.dy[i]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 n[i].v[e] *= rstd;
@@ -154,7 +169,7 @@ __global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackw
 #pragma unroll
             for (int e = 0; e < 8; ++e) dx.v[e] = rstd * __builtin_fmaf(-n[i].v[e], mean, dn[i].v[e]);
             if (g.dR) {
-                const Eight dr = load8_part<TYPE>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
+                const Eight dr = widen8<TYPE>(row.dr[i]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dx.v[e] += dr.v[e];
             }
@@ -169,26 +184,44 @@ __global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackw
     }
 }
 
-// dw[k] = sum of `rows` rows of partial.  A workgroup takes 32 columns; its 16 rows of threads add every 16th row each, two
-// columns a thread, and meet in LDS in thread-row order.
+// dw[k] = sum of `rows` rows of partial.  A workgroup takes 32 columns: 8 lanes with 4 each, 32 rows of lanes that add every
+// 32nd row (eight loads in flight each) and meet in LDS in their order.
 __global__ __launch_bounds__(256) void rmsnorm_dw_kernel(const float* __restrict__ partial, int rows, int K, float* __restrict__ dW) {
-    __shared__ float part[16][33];
-    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+    __shared__ float part[32][33];
+    const int c = threadIdx.x & 7, r = threadIdx.x >> 3;
+    const int k = (int)blockIdx.x * 32 + 4 * c;
+    const float* p = partial + (k < K ? k : 0);
+    const bool whole = k + 4 <= K;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    constexpr int AHEAD = 8;
+    for (int m0 = r; m0 < rows; m0 += 32 * AHEAD) {
+        f32x4 v[AHEAD];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int k = (int)blockIdx.x * 32 + 16 * j + c;
-        float v = 0.f;
-        if (k < K)
-            for (int m = r; m < rows; m += 16) v += partial[(size_t)m * K + k];
-        part[r][16 * j + c] = v;
+        for (int j = 0; j < AHEAD; ++j) {
+            const int m = m0 + 32 * j;
+            v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (m < rows) {
+                if (whole) {
+                    v[j] = *reinterpret_cast<const f32x4_any*>(p + (size_t)m * K);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (k + e < K) v[j][e] = p[(size_t)m * K + e];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) sum += v[j];
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[r][4 * c + e] = sum[e];
     __syncthreads();
     if (threadIdx.x < 32) {
-        const int k = (int)blockIdx.x * 32 + (int)threadIdx.x;
+        const int col = (int)blockIdx.x * 32 + (int)threadIdx.x;
         float v = part[0][threadIdx.x];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) v += part[i][threadIdx.x];
-        if (k < K) dW[k] = v;
+        for (int i = 1; i < 32; ++i) v += part[i][threadIdx.x];
+        if (col < K) dW[col] = v;
     }
 }
 
