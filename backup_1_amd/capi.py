@@ -5,6 +5,7 @@ device is not an MI355X the calls raise.
 """
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -30,7 +31,7 @@ SYMBOLS = [
     "decx_hip_b_read_extent", "decx_hip_sgemm_plan", "decx_hip_sgemm_plan_split", "decx_hip_hgemm_plan", "decx_hip_hgemm_plan_split", "decx_hip_conv_plan_split", "decx_hip_conv_patch_offsets_fit", "decx_hip_set_splitk_mode", "decx_hip_hgemm_f32acc_noalloc", "decx_hip_release_tmp", "decx_hip_tmp_malloc", "decx_hip_tmp_free",
     "decx_hip_f8_quantize", "decx_hip_f8_quantize_async", "decx_hip_f8gemm", "decx_hip_f8gemm_async", "decx_hip_rmsnorm_f8",
     "decx_hip_rmsnorm_f8_async", "decx_hip_rmsnorm_backward", "decx_hip_rmsnorm_backward_async", "decx_hip_rmsnorm_backward_workspace",
-    "decx_hip_set_f8gemm_variant", "decx_hip_f8gemm_plan",
+    "decx_hip_set_f8gemm_variant", "decx_hip_f8gemm_plan", "decx_hip_f8_call",
 ]
 
 
@@ -100,6 +101,7 @@ def lib():
         for name, args in (("f8_quantize", quantize), ("f8gemm", f8gemm_args), ("rmsnorm_f8", norm), ("rmsnorm_backward", norm_backward)):
             sig["decx_hip_" + name] = sig["decx_hip_" + name + "_async"] = (args, I)
         sig["decx_hip_rmsnorm_backward_workspace"] = ([I, I], Z)
+        sig["decx_hip_f8_call"] = ([I, P, I], I)
         sig["decx_hip_set_f8gemm_variant"] = ([I], I)
         sig["decx_hip_f8gemm_plan"] = ([I, I, I, I, I, I, ctypes.c_long, ctypes.c_long, I], I)
         for name, (args, res) in sig.items():
@@ -215,20 +217,30 @@ def conv2_im2col(dsrc, H, W, dpitch, src_row_stride, dfilt, N, kh, kw, filt_stri
              dst_row_stride, flag))
 
 
+# The 8-bit operators' arguments go through one buffer: ctypes' cost grows with their number, and it would be most of a small
+# call's time.  Like the library, not for several threads at once.  Pointers and flags are whole numbers, None a null pointer.
+_words = ctypes.create_string_buffer(8 * 20)
+_words_at = ctypes.addressof(_words)
+_pack_quantize, _pack_f8gemm = struct.Struct("=16q").pack_into, struct.Struct("=20q").pack_into
+_pack_norm, _pack_norm_backward = struct.Struct("=5qd14q").pack_into, struct.Struct("=16q").pack_into
+_CALL_F8_QUANTIZE, _CALL_F8GEMM, _CALL_RMSNORM_F8, _CALL_RMSNORM_BACKWARD = 0, 1, 2, 3
+
+
 def f8_quantize(dX, ldx, dtype, M, K, block_rows, fmt, scale_type, dQ, ldq, dS, lds, dQt=None, ldqt=0, dSt=None, ldst=0, blocking=True):
-    fn = lib().decx_hip_f8_quantize if blocking else lib().decx_hip_f8_quantize_async
-    check(fn(dX, ldx, dtype, M, K, block_rows, fmt, scale_type, dQ, ldq, dS, lds, dQt, ldqt, dSt, ldst))
+    _pack_quantize(_words, 0, dX, ldx, dtype, M, K, block_rows, fmt, scale_type, dQ or 0, ldq, dS or 0, lds, dQt or 0, ldqt, dSt or 0, ldst)
+    check((_lib or lib()).decx_hip_f8_call(_CALL_F8_QUANTIZE, _words_at, blocking))
 
 
 def f8gemm(dA, lda, fmt_a, dSA, ldsa, dB, ldb, fmt_b, dSB, ldsb, b_block_rows, scale_type, dD, ldd, dtype, M, N, K, dC=None, ldc=0,
            blocking=True):
-    fn = lib().decx_hip_f8gemm if blocking else lib().decx_hip_f8gemm_async
-    check(fn(dA, lda, fmt_a, dSA, ldsa, dB, ldb, fmt_b, dSB, ldsb, b_block_rows, scale_type, dC, ldc, dD, ldd, dtype, M, N, K))
+    _pack_f8gemm(_words, 0, dA, lda, fmt_a, dSA, ldsa, dB, ldb, fmt_b, dSB, ldsb, b_block_rows, scale_type, dC or 0, ldc, dD, ldd, dtype, M, N, K)
+    check((_lib or lib()).decx_hip_f8_call(_CALL_F8GEMM, _words_at, blocking))
 
 
 def rmsnorm_f8(dX, ldx, dR, ldr, dW, eps, dtype, M, K, dH, ldh, dRstd, dY, ldy, dQ, ldq, dS, lds, fmt=E4M3, scale_type=SCALE_F32, blocking=True):
-    fn = lib().decx_hip_rmsnorm_f8 if blocking else lib().decx_hip_rmsnorm_f8_async
-    check(fn(dX, ldx, dR, ldr, dW, eps, dtype, M, K, dH, ldh, dRstd, dY, ldy, dQ, ldq, dS, lds, fmt, scale_type))
+    _pack_norm(_words, 0, dX, ldx, dR or 0, ldr, dW, eps, dtype, M, K, dH or 0, ldh, dRstd or 0, dY or 0, ldy, dQ or 0, ldq, dS or 0, lds, fmt,
+               scale_type)
+    check((_lib or lib()).decx_hip_f8_call(_CALL_RMSNORM_F8, _words_at, blocking))
 
 
 def rmsnorm_backward_workspace(M, K):
@@ -236,8 +248,8 @@ def rmsnorm_backward_workspace(M, K):
 
 
 def rmsnorm_backward(dH, ldh, dW, dRstd, ddY, lddy, ddR, lddr, dtype, M, K, ddX, lddx, ddW, dWork, work_bytes, blocking=True):
-    fn = lib().decx_hip_rmsnorm_backward if blocking else lib().decx_hip_rmsnorm_backward_async
-    check(fn(dH, ldh, dW, dRstd, ddY, lddy, ddR, lddr, dtype, M, K, ddX, lddx, ddW, dWork, work_bytes))
+    _pack_norm_backward(_words, 0, dH, ldh, dW, dRstd, ddY, lddy, ddR or 0, lddr, dtype, M, K, ddX, lddx, ddW or 0, dWork or 0, work_bytes)
+    check((_lib or lib()).decx_hip_f8_call(_CALL_RMSNORM_BACKWARD, _words_at, blocking))
 
 
 def timer_start():

@@ -757,6 +757,38 @@ int decx_hip_rmsnorm_backward(const void* H, int ldh, const void* W, const float
     return finish(rmsnorm_backward_enqueue(H, ldh, W, rstd, dY, lddy, dR, lddr, type, M, K, dX, lddx, dW, work, work_bytes));
 }
 
+int decx_hip_f8_call(int call, const int64_t* a, int blocking) {
+    if (!a) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "null argument list\n");
+    auto ptr = [&](int i) { return reinterpret_cast<void*>((uintptr_t)a[i]); };
+    auto bytes = [&](int i) { return static_cast<uint8_t*>(ptr(i)); };
+    auto floats = [&](int i) { return static_cast<float*>(ptr(i)); };
+    auto num = [&](int i) { return (int)a[i]; };
+    int rc;
+    switch (call) {
+        case DECX_HIP_CALL_F8_QUANTIZE:
+            rc = f8_quantize_enqueue(ptr(0), num(1), num(2), num(3), num(4), num(5), num(6), num(7), bytes(8), num(9), ptr(10), num(11),
+                                     bytes(12), num(13), ptr(14), num(15));
+            break;
+        case DECX_HIP_CALL_F8GEMM:
+            rc = f8gemm_enqueue(bytes(0), num(1), num(2), ptr(3), num(4), bytes(5), num(6), num(7), ptr(8), num(9), num(10), num(11), ptr(12),
+                                num(13), ptr(14), num(15), num(16), num(17), num(18), num(19));
+            break;
+        case DECX_HIP_CALL_RMSNORM_F8: {
+            double eps;
+            memcpy(&eps, a + 5, sizeof(eps));
+            rc = rmsnorm_f8_enqueue(ptr(0), num(1), ptr(2), num(3), ptr(4), (float)eps, num(6), num(7), num(8), ptr(9), num(10), floats(11),
+                                    ptr(12), num(13), bytes(14), num(15), ptr(16), num(17), num(18), num(19));
+            break;
+        }
+        case DECX_HIP_CALL_RMSNORM_BACKWARD:
+            rc = rmsnorm_backward_enqueue(ptr(0), num(1), ptr(2), floats(3), ptr(4), num(5), ptr(6), num(7), num(8), num(9), num(10), ptr(11),
+                                          num(12), floats(13), ptr(14), (size_t)a[15]);
+            break;
+        default: return fail(DECX_HIP_FAIL_ERROR_FLAG, "unknown call\n");
+    }
+    return blocking ? finish(rc) : rc;
+}
+
 int decx_hip_tmp_malloc(void** dptr, size_t bytes) {
     if (!g_rt.is_init) return need_init();
     if (!dptr || bytes == 0) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "null pointer or empty block\n");

@@ -28,19 +28,24 @@ template <int TYPE>
 struct RawEight {
     u32x4 w[TYPE == 0 ? 2 : 1];
 };
-// Non-temporal: read once by this launch.  The streaming kernels here reach 5.0 TB/s on ordinary accesses to data that no
-// cache holds and 5.6 - 6.2 on these.
-template <int TYPE>
+// STREAM: non-temporal, for inputs that no cache can hold.  Stores are non-temporal always: written once, and by then the
+// caches are better used for what is read.
+template <int TYPE, bool STREAM = false>
 __device__ __forceinline__ RawEight<TYPE> load_raw8(const typename Wide<TYPE>::T* p) {
     RawEight<TYPE> r;
-    r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
-    if constexpr (TYPE == 0) r.w[1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p + 4));
+    if constexpr (STREAM) {
+        r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+        if constexpr (TYPE == 0) r.w[1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p + 4));
+    } else {
+        r.w[0] = *reinterpret_cast<const u32x4_any*>(p);
+        if constexpr (TYPE == 0) r.w[1] = *reinterpret_cast<const u32x4_any*>(p + 4);
+    }
     return r;
 }
 // the first `n` of 8 elements (n may be <= 0 or > 8), the others 0; reads nothing beyond them
-template <int TYPE>
+template <int TYPE, bool STREAM = false>
 __device__ __forceinline__ RawEight<TYPE> load_raw8_part(const typename Wide<TYPE>::T* p, int n) {
-    if (n >= 8) return load_raw8<TYPE>(p);
+    if (n >= 8) return load_raw8<TYPE, STREAM>(p);
     RawEight<TYPE> r = {};
 #pragma unroll
     for (int e = 0; e < 8; ++e)

@@ -108,6 +108,7 @@ struct RmsNormBackwardArgs {
     float* partial;           // [workgroups][K], nullptr: no dW wanted
     size_t ldh, lddy, lddr, lddx;
     int M, K, rows_each;
+    int stream;               // the inputs are larger than the memory-side cache
 };
 
 // Workgroup b owns rows b * rows_each ...: their dx, and their part of dw in a row of `partial`, which the second kernel
@@ -128,15 +129,20 @@ __global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackw
         RawEight<TYPE> h[CH], dy[CH], dr[CH];
         float rstd;
     };
-    auto load_row = [&](Row& r, int m) {
+    auto load_row_as = [&](Row& r, int m, auto stream_tag) {
+        constexpr bool STREAM = decltype(stream_tag)::value;
         r.rstd = g.rstd[m];
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            r.h[i] = load_raw8_part<TYPE>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k);
-            r.dy[i] = load_raw8_part<TYPE>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k);
-            if (g.dR) r.dr[i] = load_raw8_part<TYPE>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
+            r.h[i] = load_raw8_part<TYPE, STREAM>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k);
+            r.dy[i] = load_raw8_part<TYPE, STREAM>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k);
+            if (g.dR) r.dr[i] = load_raw8_part<TYPE, STREAM>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
         }
+    };
+    auto load_row = [&](Row& r, int m) {
+        if (TYPE != 0 && g.stream) load_row_as(r, m, std::true_type{});
+        else load_row_as(r, m, std::false_type{});
     };
     Row next;
     load_row(next, first);
@@ -184,21 +190,22 @@ __global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackw
     }
 }
 
-// dw[k] = sum of `rows` rows of partial.  A workgroup takes 32 columns: 8 lanes with 4 each, 32 rows of lanes that add every
-// 32nd row (eight loads in flight each) and meet in LDS in their order.
+// dw[k] = sum of `rows` rows of partial.  A workgroup takes COLS columns: COLS / 4 lanes with 4 each, 1024 / COLS rows of
+// lanes that add every (1024 / COLS)th row, eight loads in flight each, and meet in LDS in their order.
+template <int COLS>
 __global__ __launch_bounds__(256) void rmsnorm_dw_kernel(const float* __restrict__ partial, int rows, int K, float* __restrict__ dW) {
-    __shared__ float part[32][33];
-    const int c = threadIdx.x & 7, r = threadIdx.x >> 3;
-    const int k = (int)blockIdx.x * 32 + 4 * c;
+    constexpr int LANES = COLS / 4, GROUPS = 256 / LANES, AHEAD = 8;
+    __shared__ float part[GROUPS][COLS + 1];
+    const int c = threadIdx.x % LANES, r = threadIdx.x / LANES;
+    const int k = (int)blockIdx.x * COLS + 4 * c;
     const float* p = partial + (k < K ? k : 0);
     const bool whole = k + 4 <= K;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    constexpr int AHEAD = 8;
-    for (int m0 = r; m0 < rows; m0 += 32 * AHEAD) {
+    for (int m0 = r; m0 < rows; m0 += GROUPS * AHEAD) {
         f32x4 v[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            const int m = m0 + 32 * j;
+            const int m = m0 + GROUPS * j;
             v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (m < rows) {
                 if (whole) {
@@ -216,12 +223,18 @@ __global__ __launch_bounds__(256) void rmsnorm_dw_kernel(const float* __restrict
 #pragma unroll
     for (int e = 0; e < 4; ++e) part[r][4 * c + e] = sum[e];
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int col = (int)blockIdx.x * 32 + (int)threadIdx.x;
-        float v = part[0][threadIdx.x];
+    // 8 threads a column add GROUPS / 8 rows of lanes each, then one of them the 8
+    constexpr int SHARE = GROUPS / 8;
+    static_assert(COLS * 8 <= 256 && GROUPS % 8 == 0, "8 threads a column");
+    const int col = threadIdx.x / 8, share = threadIdx.x % 8;
+    if (col < COLS) {
+        float v = part[share * SHARE][col];
 #pragma unroll
-        for (int i = 1; i < 32; ++i) v += part[i][threadIdx.x];
-        if (col < K) dW[col] = v;
+        for (int i = 1; i < SHARE; ++i) v += part[share * SHARE + i][col];
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) v += __shfl_xor(v, d);
+        const int at = (int)blockIdx.x * COLS + col;
+        if (share == 0 && at < K) dW[at] = v;
     }
 }
 
@@ -231,6 +244,7 @@ constexpr int kRmsNormMaxK = 32768;       // 1024 threads with 4 chunks each hol
 #define DECX_RMSNORM_SHAPES(K, LAUNCH)       \
     do {                                     \
         if ((K) <= 512) LAUNCH(64, 1);       \
+        else if ((K) <= 1024) LAUNCH(128, 1); \
         else if ((K) <= 2048) LAUNCH(256, 1); \
         else if ((K) <= 4096) LAUNCH(256, 2); \
         else if ((K) <= 8192) LAUNCH(256, 4); \
@@ -281,14 +295,18 @@ int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const voi
     return rmsnorm_f8_launch<2>(g);
 }
 
-// workgroups of the gradient: two for each compute unit, or one for each row
-static int rmsnorm_backward_groups(int M) {
-    const int most = 2 * (g_rt.compute_units > 0 ? g_rt.compute_units : 256);
+// Workgroups of the gradient: as many as keep about 32 KB of each input on a compute unit, 2 to 8 a unit (short rows wait for
+// memory one after the other: 8192 x 256 took 24 us with 2, 17.5 with 8; long fp32 ones gain nothing: 8192 x 4096 114 us
+// with 2, 123 with 4), and none without rows.  The workspace is sized for the 2-byte types.
+static int rmsnorm_backward_groups(int M, int K, int size) {
+    const int held = K <= 512 ? 512 : K <= 1024 ? 1024 : K <= 2048 ? 2048 : K <= 4096 ? 4096 : 8192;
+    const int fit = 32768 / (held * size), each = fit < 2 ? 2 : fit > 8 ? 8 : fit;
+    const int most = each * (g_rt.compute_units > 0 ? g_rt.compute_units : 256);
     const int groups = M < most ? M : most;
-    return cdiv(M, cdiv(M, groups));                            // none without rows
+    return cdiv(M, cdiv(M, groups));
 }
 
-size_t rmsnorm_backward_workspace(int M, int K) { return (size_t)rmsnorm_backward_groups(M) * K * sizeof(float); }
+size_t rmsnorm_backward_workspace(int M, int K) { return (size_t)rmsnorm_backward_groups(M, K, 2) * K * sizeof(float); }
 
 int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR, int lddr,
                              int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes) {
@@ -306,15 +324,21 @@ int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float*
     if (dW && (!work || (reinterpret_cast<uintptr_t>(work) & 3u) || work_bytes < rmsnorm_backward_workspace(M, K)))
         return fail(DECX_HIP_FAIL_ERROR_PARAMS, "the weight's gradient needs a workspace of %zu bytes (decx_hip_rmsnorm_backward_workspace)\n",
                     rmsnorm_backward_workspace(M, K));
-    const int groups = rmsnorm_backward_groups(M);
+    const int groups = rmsnorm_backward_groups(M, K, type == DECX_HIP_F32 ? 4 : 2);
     RmsNormBackwardArgs g = {};
     g.H = H, g.W = W, g.dY = dY, g.dR = dR, g.rstd = rstd, g.dX = dX, g.partial = dW ? static_cast<float*>(work) : nullptr;
     g.ldh = (size_t)ldh, g.lddy = (size_t)lddy, g.lddr = (size_t)lddr, g.lddx = (size_t)lddx;
     g.M = M, g.K = K, g.rows_each = cdiv(M, groups);
+    // 16-bit inputs of more than the memory-side cache's 256 MiB are read past the caches: 8192 x 8192, 402 MB, 104 us
+    // against 112; 8192 x 1000, 49 MB, 36 against 31 (and in fp32, whose lanes read a line in two pieces, always slower)
+    g.stream = (size_t)M * K * (dR ? 6 : 4) > ((size_t)256 << 20);
     int rc = type == DECX_HIP_F32 ? rmsnorm_backward_launch<0>(g, groups)
                                   : type == DECX_HIP_F16 ? rmsnorm_backward_launch<1>(g, groups) : rmsnorm_backward_launch<2>(g, groups);
     if (rc || !dW) return rc;
-    hipLaunchKernelGGL(rmsnorm_dw_kernel, dim3((unsigned)cdiv(K, 32)), dim3(256), 0, g_rt.stream, g.partial, groups, K, dW);
+    if (K <= 2048)          // narrow pieces where wide ones would leave most of the chip idle
+        hipLaunchKernelGGL(rmsnorm_dw_kernel<8>, dim3((unsigned)cdiv(K, 8)), dim3(256), 0, g_rt.stream, g.partial, groups, K, dW);
+    else
+        hipLaunchKernelGGL(rmsnorm_dw_kernel<32>, dim3((unsigned)cdiv(K, 32)), dim3(256), 0, g_rt.stream, g.partial, groups, K, dW);
     HIP_TRY(hipGetLastError());
     return 0;
 }

@@ -325,6 +325,15 @@ int decx_hip_rmsnorm_backward(const void* H, int ldh, const void* W, const float
 int decx_hip_rmsnorm_backward_async(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR,
                                     int lddr, int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes);
 
+/* The four calls above with their arguments, in their order, in an array of 64-bit integers (eps as the bits of a double):
+ * for bindings whose cost grows with the number of arguments -- ctypes takes 2.6 us for twenty, 0.8 this way, of calls
+ * that take the GPU 4.  blocking = 0: the _async form. */
+#define DECX_HIP_CALL_F8_QUANTIZE      0
+#define DECX_HIP_CALL_F8GEMM           1
+#define DECX_HIP_CALL_RMSNORM_F8       2
+#define DECX_HIP_CALL_RMSNORM_BACKWARD 3
+int decx_hip_f8_call(int call, const int64_t* arguments, int blocking);
+
 /* de::release_all_tmp (core/memory_management/Memory_pool.h:23-37: releases the blocks its memory pools hold).  The
  * host-matrix entry points (decx_hip_gemm_host_*, decx_hip_gemm3_host_*) keep their device blocks for the next call, as
  * the reference's device pool does (MemoryPool_D.h); this waits for the device and frees them. */

@@ -245,3 +245,35 @@ def test_refusals(gpu):
     refused(0x0d, D=d.ptr + 65538)
     refused(0x0d, D=d.ptr + 65537, type=capi.BF16)
     refused(0x0d, SA=d.ptr + 8193)
+
+
+def test_plain_and_packed_entry_points_agree(gpu):
+    """The tests call through capi.py, that is decx_hip_f8_call; here each operator through its own entry point too."""
+    L = capi.lib()
+    M, K, N = 33, 272, 48
+    x = workloads.normal((M, K), 81).astype(np.float32)
+    w = workloads.normal((K,), 82).astype(np.float32)
+    b, sb = real_operand(N, K, capi.E4M3, capi.SCALE_F32, 128, 83)
+    dx, dw, dB, dSB = Pitched(x), Pitched(w), Pitched(b), Pitched(sb)
+
+    def outputs():
+        return [Pitched.empty(M, K, np.uint8), Pitched.empty(3, M, np.float32), Pitched.empty(M, N, np.float32), Pitched.empty(M, K, np.float32),
+                Pitched.empty(1, M, np.float32), Pitched.empty(M, K, np.float32), Pitched.empty(1, K, np.float32)]
+
+    need = capi.rmsnorm_backward_workspace(M, K)
+    work = capi.DeviceBuffer(need)
+    p, o = outputs(), outputs()
+    for (q, s, d, y, r, dX, dW), direct in ((p, True), (o, False)):
+        if direct:
+            capi.check(L.decx_hip_rmsnorm_f8(dx.ptr, K, None, 0, dw.ptr, 1e-5, 0, M, K, None, 0, r.ptr, y.ptr, K, None, 0, None, 0, 0, 0))
+            capi.check(L.decx_hip_f8_quantize(y.ptr, K, 0, M, K, 1, 0, 0, q.ptr, K, s.ptr, M, None, 0, None, 0))
+            capi.check(L.decx_hip_f8gemm(q.ptr, K, 0, s.ptr, M, dB.ptr, K, 0, dSB.ptr, dSB.ld, 128, 0, None, 0, d.ptr, N, 0, M, N, K))
+            capi.check(L.decx_hip_rmsnorm_backward(dx.ptr, K, dw.ptr, r.ptr, y.ptr, K, None, 0, 0, M, K, dX.ptr, K, dW.ptr, work.ptr, need))
+        else:                                                    # without waiting in between: one stream, in order
+            capi.rmsnorm_f8(dx.ptr, K, None, 0, dw.ptr, 1e-5, 0, M, K, None, 0, r.ptr, y.ptr, K, None, 0, None, 0, blocking=False)
+            capi.f8_quantize(y.ptr, K, 0, M, K, 1, 0, 0, q.ptr, K, s.ptr, M, blocking=False)
+            capi.f8gemm(q.ptr, K, 0, s.ptr, M, dB.ptr, K, 0, dSB.ptr, dSB.ld, 128, 0, d.ptr, N, 0, M, N, K, blocking=False)
+            capi.rmsnorm_backward(dx.ptr, K, dw.ptr, r.ptr, y.ptr, K, None, 0, 0, M, K, dX.ptr, K, dW.ptr, work.ptr, need, blocking=False)
+            capi.sync()
+    for a, c in zip(p, o):
+        assert np.array_equal(a.result().view(np.uint8), c.result().view(np.uint8))
