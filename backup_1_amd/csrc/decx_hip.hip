@@ -851,7 +851,7 @@ int decx_hip_set_f8gemm_variant(int variant) {
 }
 int decx_hip_f8gemm_plan(int M, int N, int K, int type, int scale_type, int b_block_rows, long lda, long ldb, int aligned) {
     if (M <= 0 || N <= 0 || K <= 0 || lda < K || ldb < K) return -1;
-    return f8gemm_plan(M, N, type, scale_type, b_block_rows, lda, ldb, aligned != 0);
+    return f8gemm_plan(M, N, K, type, scale_type, b_block_rows, lda, ldb, aligned != 0);
 }
 
 int decx_hip_set_splitk_mode(int mode) {

@@ -6,11 +6,12 @@
 
 namespace decx_hip {
 
-typedef F8StreamShape<1, 1, 8, 4> F8Token;         // a token to 16 rows
-typedef F8StreamShape<4, 2, 8, 1> F8Rows;
-
-typedef F8TileShape<256, 256, 2, 4> F8TileLarge;   // 8 waves of 128 x 64, two a SIMD
+typedef F8StreamShape<1, 1, 8, 2> F8Stream16x16;
+typedef F8StreamShape<2, 1, 8, 2> F8Stream32x16;
+typedef F8StreamShape<4, 2, 8, 1> F8Stream64x32;
+typedef F8StreamShape<4, 4, 8, 1> F8Stream64x64;
 typedef F8TileShape<128, 128, 2, 2> F8TileSmall;   // 4 waves of 64 x 64, two workgroups a CU
+typedef F8TileShape<256, 256, 2, 4> F8TileLarge;   // 8 waves of 128 x 64, two a SIMD
 
 template <class S, class F>
 static int launch_f8gemm_tile(F8GemmArgs g) {
@@ -32,6 +33,11 @@ static int launch_f8gemm_tile(F8GemmArgs g) {
 template <class S, class F>
 static int launch_f8gemm_stream(F8GemmArgs g) {
     auto kern = f8gemm_stream_kernel<S, F>;
+    static bool attr_done = false;
+    if (!attr_done) {
+        HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS_BYTES));
+        attr_done = true;
+    }
     g.tiles_m = cdiv(g.M, S::BM), g.tiles_n = cdiv(g.N, S::BN);
     const long total = (long)g.tiles_m * g.tiles_n;
     if (total > 0x7fffffffL) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
@@ -44,9 +50,13 @@ static int launch_f8gemm_stream(F8GemmArgs g) {
 template <class F>
 static int launch_f8gemm(const F8GemmArgs& g) {
     switch (g.variant) {
-        case 1: return launch_f8gemm_stream<F8Token, F>(g);
-        case 2: return launch_f8gemm_stream<F8Rows, F>(g);
-        case 3: return launch_f8gemm_tile<F8TileSmall, F>(g);
+        case 1: return launch_f8gemm_stream<F8Stream16x16, F>(g);
+        case 2: return launch_f8gemm_stream<F8Stream32x16, F>(g);
+        case 3: return launch_f8gemm_stream<F8Stream64x32, F>(g);
+        case 4:
+            if constexpr (!F::EXACT) return launch_f8gemm_stream<F8Stream64x64, F>(g);
+            return launch_f8gemm_stream<F8Stream64x32, F>(g);
+        case 5: return launch_f8gemm_tile<F8TileSmall, F>(g);
         default:
             if constexpr (!F::EXACT && !F::B_PER_ROW) return launch_f8gemm_tile<F8TileLarge, F>(g);
             return launch_f8gemm_tile<F8TileSmall, F>(g);

@@ -112,7 +112,7 @@ int f8_quantize_enqueue(const void* X, int ldx, int type, int M, int K, int bloc
 int f8gemm_enqueue(const uint8_t* A, int lda, int format_a, const void* SA, int ldsa, const uint8_t* B, int ldb, int format_b,
                    const void* SB, int ldsb, int b_block_rows, int scale_type, const void* Cin, int ldc, void* D, int ldd, int type, int M,
                    int N, int K);
-int f8gemm_plan(int M, int N, int type, int scale_type, int b_block_rows, long lda, long ldb, bool aligned);
+int f8gemm_plan(int M, int N, int K, int type, int scale_type, int b_block_rows, long lda, long ldb, bool aligned);
 int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H, int ldh,
                        float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type);
 size_t rmsnorm_backward_workspace(int M, int K);

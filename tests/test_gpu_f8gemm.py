@@ -96,7 +96,7 @@ def test_formats_and_scales(gpu, fa, fb, scale, b_rows, M, N, K):
     check(a, sa, fa, b, sb, fb, b_rows, capi.BF16, C=ref.to_type(workloads.normal((M, N), 3), capi.BF16), pitch=(align, align, 0, 0, 0))
 
 
-VARIANTS = (1, 2, 3, 4)
+VARIANTS = (1, 2, 3, 4, 5, 6)
 
 
 @pytest.fixture
