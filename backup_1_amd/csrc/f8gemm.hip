@@ -11,12 +11,12 @@ namespace decx_hip {
 //   5: 128 x 128 LDS-DMA tiles (f8gemm_tile.hpp), 6: 256 x 256; both need `aligned` operands, the latter not the exact sums
 //      of fp32 results nor an fp32 scale for each row of B
 // The cheapest by a model of what was measured on an MI355X, in us:
-//   1 - 4: a CU takes in 81 KB a us once 1.5 us have passed, a workgroup's share of A and B, as many workgroups after each
-//          other as a CU has of them (exact sums a third more, an fp32 scale for each row of B half more in 4); and B passes
+//   1 - 4: a CU takes in 81 KB a us, a workgroup's share of A and B, once 1.5 us have passed, and again (at most 1.5 us) for
+//          each of the workgroups that a CU has after each other (exact sums a third more, an fp32 scale for each row of B half more in 4); and B passes
 //          through at 6.5 MB a us at most
 //   5: 0.64 a block of K while a CU has one tile, 1 for two; exact sums 1.15 and 2.2
 //   6: 1.05 a block of K on a nearly empty chip to 1.47 on a full one
-//   plus 2.4 (1 - 4), 3 (5) and 7 to 11 (6) for the launch, the first loads and the store.
+//   plus 2.4 (1 - 4), 3 and half of the store (5) and 7 to 11 (6) for the launch, the first loads and the store.
 // On 74 shapes from 1 x 4096 x 4096 to 4096^3, bf16 and fp32 results: within 5 % of the best kernel on all but three.
 static int plan_f8gemm(int M, int N, int K, int type, int scale_type, int b_block_rows, bool aligned, bool large) {
     const int forced = g_rt.f8gemm_variant;
@@ -30,13 +30,15 @@ static int plan_f8gemm(int M, int N, int K, int type, int scale_type, int b_bloc
     for (int v = 1; v <= (exact ? 3 : 4); ++v) {
         const int mi = MI[v - 1], ni = NI[v - 1];
         const double rounds = std::ceil((double)cdiv(M, 16 * mi) * cdiv(N, 16 * ni) / cus), slower = exact ? 1.35 : row_scales && v == 4 ? 1.5 : 1.0;
-        const double taken = rounds * (1.5 + (mi + ni) * 16.0 * K * slower / 81e3), passed = (double)N * K / 6.5e6;
+        const double share = (mi + ni) * 16.0 * K * slower / 81e3, passed = (double)N * K / 6.5e6;
+        const double taken = 1.5 + rounds * share + (rounds - 1) * (share < 1.5 ? share : 1.5);
         const double cost = 2.4 + (taken > passed ? taken : passed);
         if (v == 1 || cost < least) best = v, least = cost;
     }
     if (!aligned) return best;
     const double small = (double)cdiv(M, 128) * cdiv(N, 128), big = (double)cdiv(M, 256) * cdiv(N, 256);
-    const double cost5 = 3.0 + blocks * (small <= cus ? (exact ? 1.15 : 0.64) : std::ceil(small / (2 * cus)) * (exact ? 2.2 : 1.0));
+    const double store = 0.5 * (double)M * N * (exact ? 4 : 2) / 5e6;
+    const double cost5 = 3.0 + store + blocks * (small <= cus ? (exact ? 1.15 : 0.64) : std::ceil(small / (2 * cus)) * (exact ? 2.2 : 1.0));
     if (cost5 < least) best = 5, least = cost5;
     const double fill = big < cus ? big / cus : 1.0;
     const double cost6 = 7.0 + 4.0 * fill + blocks * std::ceil(big / cus) * (1.05 + 0.42 * fill);

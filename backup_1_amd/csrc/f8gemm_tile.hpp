@@ -185,6 +185,12 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
     };
     F16Fragment wide_b[NI], wide_a[UM];
     float row_scale[UM], col_scale = 0.f;
+    // EXACT: B is converted as it comes in, columns 0 and 1 of a step during the last unit of the step before (theirs are done
+    // by then), the others before their first product: 128 conversions a step among 64 matrix instructions, evenly
+    auto widen_b = [&](auto ni_tag) {
+        constexpr int NIX = decltype(ni_tag)::value;
+        wide_b[NIX] = f8_widen<F::FB>(f8_fragment(bf[NIX].lo, bf[NIX].hi));
+    };
     auto mfma_one = [&](auto u_tag, auto i_tag) {
         constexpr int U = decltype(u_tag)::value, I = decltype(i_tag)::value, NIX = I >> 1, ROW = (I & 1) ^ (NIX & 1), SET = U & 1;
         constexpr int N = U * BLK + I;
@@ -200,7 +206,7 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
                     if constexpr (EXACT) wide_a[r] = f8_widen<F::FA>(f8_fragment(af[SET][r].lo, af[SET][r].hi));
                 }
             }
-            if constexpr (EXACT && U == 0 && (I & 1) == 0) wide_b[NIX] = f8_widen<F::FB>(f8_fragment(bf[NIX].lo, bf[NIX].hi));
+            if constexpr (EXACT && U == 0 && (I & 1) == 0 && NIX >= 2) widen_b(std::integral_constant<int, NIX>{});
             Pending& p = pending[N % RING];
             if constexpr (EXACT) p.sum = f8_mfma_exact(wide_b[NIX], wide_a[ROW]);
             else p.sum = f8_mfma<F::FA, F::FB>(f8_fragment(bf[NIX].lo, bf[NIX].hi), f8_fragment(af[SET][ROW].lo, af[SET][ROW].hi), f32x4{0.f, 0.f, 0.f, 0.f});
@@ -258,6 +264,7 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
             for (int r = 0; r < UM; ++r) af[0][r].lo &= keep_lo, af[0][r].hi &= keep_hi;
 #pragma unroll
             for (int ni = 0; ni < NI; ++ni) bf[ni].lo &= keep_lo, bf[ni].hi &= keep_hi;
+            if constexpr (EXACT) widen_b(I0{}), widen_b(std::integral_constant<int, 1>{});
         }
         inner_units(stage_tag, ragged_tag, keep_lo, keep_hi);
         mfma_one(Last{}, I0{});
@@ -280,6 +287,7 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
             }
             static_for<(I * S::LOADS) / SLOTS, ((I + 1) * S::LOADS) / SLOTS>([&](auto j_tag) { issue_one(stage_tag, j_tag); });
             mfma_one(Last{}, std::integral_constant<int, I + 2>{});
+            if constexpr (EXACT && (I == 3 || I == 5)) widen_b(std::integral_constant<int, (I - 3) / 2>{});
             DECX_PIN();
         });
         read_b(Next{}, std::integral_constant<int, NI - 1>{});
