@@ -42,11 +42,40 @@ __device__ __forceinline__ RawEight<TYPE> load_raw8(const typename Wide<TYPE>::T
     }
     return r;
 }
-// the first `n` of 8 elements (n may be <= 0 or > 8), the others 0; reads nothing beyond them
-template <int TYPE, bool STREAM = false>
-__device__ __forceinline__ RawEight<TYPE> load_raw8_part(const typename Wide<TYPE>::T* p, int n) {
+// 16 bytes moved down by n of them (0 < n < 16), zeros from above
+__device__ __forceinline__ u32x4 bytes_down(u32x4 v, int n) {
+    uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+    if (n >= 8) lo = hi, hi = 0, n -= 8;
+    if (n > 0) lo = lo >> (8 * n) | hi << (64 - 8 * n), hi >>= 8 * n;
+    return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+// The first `n` of 8 elements of a row (n may be <= 0 or > 8), the others 0; `at` elements of the row lie before them.  Reads
+// nothing beyond the n: what is left of a row is fetched as the row's last 8 elements, which costs one load instead of n.
+// WHOLE: n is at least 8 or at most 0 (the row's length is a multiple of 8), which keeps the loads of a row together.
+template <int TYPE, bool STREAM = false, bool WHOLE = false>
+__device__ __forceinline__ RawEight<TYPE> load_raw8_part(const typename Wide<TYPE>::T* p, int n, int at) {
     if (n >= 8) return load_raw8<TYPE, STREAM>(p);
     RawEight<TYPE> r = {};
+    if (WHOLE || n <= 0) return r;
+    if (at >= 8) {
+        r = load_raw8<TYPE, STREAM>(p + (n - 8));
+        if constexpr (TYPE == 0) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = r.w[e >> 2][e & 3];
+#pragma unroll
+            for (int s = 4; s > 0; s >>= 1)
+                if ((8 - n) & s) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = e + s < 8 ? w[e + s < 8 ? e + s : 0] : 0u;
+                }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r.w[e >> 2][e & 3] = w[e];
+        } else {
+            r.w[0] = bytes_down(r.w[0], 2 * (8 - n));
+        }
+        return r;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (e < n) {
@@ -69,8 +98,10 @@ __device__ __forceinline__ Eight widen8(const RawEight<TYPE>& raw) {
     }
     return r;
 }
-template <int TYPE>
-__device__ __forceinline__ Eight load8_part(const typename Wide<TYPE>::T* p, int n) { return widen8<TYPE>(load_raw8_part<TYPE>(p, n)); }
+template <int TYPE, bool WHOLE = false>
+__device__ __forceinline__ Eight load8_part(const typename Wide<TYPE>::T* p, int n, int at) {
+    return widen8<TYPE>(load_raw8_part<TYPE, false, WHOLE>(p, n, at));
+}
 // rounds to nearest even, once
 template <int TYPE>
 __device__ __forceinline__ void store8_part(typename Wide<TYPE>::T* p, const Eight& x, int n) {

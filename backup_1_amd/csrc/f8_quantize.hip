@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void f8_quantize_rows_kernel(const typename Wi
 #pragma unroll
     for (int j = 0; j < kQuantCols; ++j) {
         const int k = (kb0 + j) * kScaleBlock + 8 * li;
-        x[j] = load8_part<TYPE>(X + row * ldx + (k < K ? k : 0), K - k);
+        x[j] = load8_part<TYPE>(X + row * ldx + (k < K ? k : 0), K - k, k);
     }
     const int blocks = (K + kScaleBlock - 1) / kScaleBlock;
 #pragma unroll
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void f8_quantize_tile_kernel(const typename Wi
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const bool live = m0 + i < M;
-        x[i] = load8_part<TYPE>(X + (size_t)(live ? m0 + i : 0) * ldx + (k0 < K ? k0 : 0), live ? K - k0 : 0);
+        x[i] = load8_part<TYPE>(X + (size_t)(live ? m0 + i : 0) * ldx + (k0 < K ? k0 : 0), live ? K - k0 : 0, k0);
     }
     BlockScale square;
     if (SQUARE) {

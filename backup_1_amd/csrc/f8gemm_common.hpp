@@ -102,11 +102,13 @@ __device__ __forceinline__ float e8m0_value(uint32_t e) {
 __device__ __forceinline__ i32x8 f8_fragment(u32x4 lo, u32x4 hi) {
     return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
-// a 16-byte unit of which only the first n codes exist (n may be <= 0 or >= 16): the others are zeros, whose products add
-// nothing whatever the block's scale (but infinity); nothing beyond the n is read
-__device__ __forceinline__ u32x4 f8_unit_part(const uint8_t* p, int n) {
+// a 16-byte unit of which only the first n codes exist (n may be <= 0 or >= 16), `at` of the row's codes before it: the others
+// are zeros, whose products add nothing whatever the block's scale (but infinity); nothing beyond the n is read
+__device__ __forceinline__ u32x4 f8_unit_part(const uint8_t* p, int n, int at) {
     if (n >= 16) return *reinterpret_cast<const u32x4_any*>(p);
     u32x4 v = {0u, 0u, 0u, 0u};
+    if (n <= 0) return v;
+    if (at >= 16) return bytes_down(*reinterpret_cast<const u32x4_any*>(p + (n - 16)), 16 - n);
 #pragma unroll
     for (int e = 0; e < 16; ++e)
         if (e < n) v[e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));

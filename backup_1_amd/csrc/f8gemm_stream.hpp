@@ -101,7 +101,7 @@ __global__ __launch_bounds__(S::NT) void f8gemm_stream_kernel(const F8GemmArgs g
         const size_t at = (size_t)kb * kScaleBlock;
         const int left = g.K - kb * kScaleBlock - 16 * unit;    // codes of this lane's unit and after it
         auto load = [&](const uint8_t* p) -> u32x4 {
-            if constexpr (decltype(ragged_tag)::value) return f8_unit_part(p, left);
+            if constexpr (decltype(ragged_tag)::value) return f8_unit_part(p, left, g.K - left);
             else return *reinterpret_cast<const u32x4_any*>(p);
         };
 #pragma unroll

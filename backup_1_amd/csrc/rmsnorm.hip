@@ -53,20 +53,27 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
     const int K = g.K, m = xcd_row((int)blockIdx.x, g.M);
     const T* x = static_cast<const T*>(g.X) + (size_t)m * g.ldx;
     Eight h[CH];
+    auto load_sum = [&](auto whole_tag) {
+        constexpr bool WHOLE = decltype(whole_tag)::value;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+            h[i] = load8_part<TYPE, WHOLE>(x + at, K - k, k);
+            if (g.R) {
+                const Eight r = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k, k);
+                // the sum is what the stream carries on, so it is rounded to its type here and the norm is taken of that
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[i].v[e] = (float)(T)(h[i].v[e] + r.v[e]);
+            }
+        }
+    };
+    if (K % 8 == 0) load_sum(std::true_type{});
+    else load_sum(std::false_type{});
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-        h[i] = load8_part<TYPE>(x + at, K - k);
-        if (g.R) {
-            const Eight r = load8_part<TYPE>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k);
-            // the sum is what the stream carries on, so it is rounded to its type here and the norm is taken of that
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[i].v[e] = (float)(T)(h[i].v[e] + r.v[e]);
-        }
+    for (int i = 0; i < CH; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(h[i].v[e], h[i].v[e], sum);
-    }
     if (g.H) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
@@ -80,7 +87,7 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-        const Eight w = load8_part<TYPE>(static_cast<const T*>(g.W) + at, K - k);
+        const Eight w = load8_part<TYPE>(static_cast<const T*>(g.W) + at, K - k, k);
         Eight y;
 #pragma unroll
         for (int e = 0; e < 8; ++e) y.v[e] = TYPE == 0 ? h[i].v[e] * rstd * w.v[e] : h[i].v[e] * w.v[e] * rstd;     // 16-bit h * w is exact
@@ -105,18 +112,69 @@ struct RmsNormBackwardArgs {
     const void *H, *W, *dY, *dR;
     const float* rstd;
     void* dX;
-    float* partial;           // [workgroups][K], nullptr: no dW wanted
+    float* partial;           // [workgroups][K], nullptr: dW not wanted, or made by the column workgroups
+    float* dW;                // of the column workgroups
+    int row_groups;           // workgroups of rows; those behind them take columns of dW
     size_t ldh, lddy, lddr, lddx;
     int M, K, rows_each;
     int stream;               // the inputs are larger than the memory-side cache
 };
 
+// dw of some columns straight from H and dY, in workgroups of their own beside those of the rows: both are read twice, but
+// there is one launch and no workspace.  For few rows of inputs that the caches hold (rmsnorm_backward_enqueue).  64 rows a
+// pass and four passes in flight; columns for that many lanes.
+constexpr int dw_columns(int nt) { return nt / 8 < 64 ? nt / 8 : 64; }
+template <int TYPE, int NT, bool WHOLE>
+__device__ __forceinline__ void rmsnorm_dw_columns(const RmsNormBackwardArgs& g, int group) {
+    typedef typename Wide<TYPE>::T T;
+    constexpr int COLS = dw_columns(NT), LANES = COLS / 8, GROUPS = NT / LANES, AHEAD = 4;
+    __shared__ float part[GROUPS][COLS + 1];
+    const int k0 = group * COLS, c = threadIdx.x % LANES, r = threadIdx.x / LANES, k = k0 + 8 * c, at = k < g.K ? k : 0;
+    float sum[8] = {};
+    for (int m0 = r; m0 < g.M; m0 += GROUPS * AHEAD) {
+        RawEight<TYPE> h[AHEAD], dy[AHEAD];
+        float rstd[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int m = m0 + GROUPS * j, row = m < g.M ? m : 0;
+            rstd[j] = m < g.M ? g.rstd[row] : 0.f;
+            h[j] = load_raw8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.H) + (size_t)row * g.ldh + at, m < g.M ? g.K - k : 0, k);
+            dy[j] = load_raw8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.dY) + (size_t)row * g.lddy + at, m < g.M ? g.K - k : 0, k);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const Eight hv = widen8<TYPE>(h[j]), yv = widen8<TYPE>(dy[j]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] = __builtin_fmaf(yv.v[e], hv.v[e] * rstd[j], sum[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[r][8 * c + e] = sum[e];
+    __syncthreads();
+    // 8 threads a column add a share of the rows of lanes each, then meet
+    constexpr int SHARE = GROUPS / 8;
+    static_assert(COLS * 8 <= NT && GROUPS % 8 == 0, "8 threads a column");
+    const int col = threadIdx.x / 8, share = threadIdx.x % 8;
+    if (col < COLS) {
+        float v = part[share * SHARE][col];
+#pragma unroll
+        for (int i = 1; i < SHARE; ++i) v += part[share * SHARE + i][col];
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) v += __shfl_xor(v, d);
+        if (share == 0 && k0 + col < g.K) g.dW[k0 + col] = v;
+    }
+}
+
 // Workgroup b owns rows b * rows_each ...: their dx, and their part of dw in a row of `partial`, which the second kernel
 // adds up in row order (no atomics: the same bits on every run).
-template <int TYPE, int NT, int CH>
-__global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackwardArgs g) {
+template <int TYPE, int NT, int CH, bool WHOLE>
+__global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward_kernel(const RmsNormBackwardArgs g) {
     typedef typename Wide<TYPE>::T T;
     __shared__ float part[2][NT / kWave];
+    if ((int)blockIdx.x >= g.row_groups) {
+        rmsnorm_dw_columns<TYPE, NT, WHOLE>(g, (int)blockIdx.x - g.row_groups);
+        return;
+    }
     const int K = g.K, first = (int)blockIdx.x * g.rows_each;
     const int last = first + g.rows_each < g.M ? first + g.rows_each : g.M;
     Eight dw[CH];
@@ -135,9 +193,9 @@ __global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackw
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            r.h[i] = load_raw8_part<TYPE, STREAM>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k);
-            r.dy[i] = load_raw8_part<TYPE, STREAM>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k);
-            if (g.dR) r.dr[i] = load_raw8_part<TYPE, STREAM>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
+            r.h[i] = load_raw8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k, k);
+            r.dy[i] = load_raw8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k, k);
+            if (g.dR) r.dr[i] = load_raw8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k, k);
         }
     };
     auto load_row = [&](Row& r, int m) {
@@ -155,7 +213,7 @@ __global__ __launch_bounds__(NT) void rmsnorm_backward_kernel(const RmsNormBackw
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            const Eight w = load8_part<TYPE>(static_cast<const T*>(g.W) + at, K - k);
+            const Eight w = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.W) + at, K - k, k);
             n[i] = widen8<TYPE>(row.h[i]);
             dn[i] = widen8<TYPE>(row.dy[i]);
 #pragma unroll
@@ -240,30 +298,35 @@ __global__ __launch_bounds__(256) void rmsnorm_dw_kernel(const float* __restrict
 
 constexpr int kRmsNormMaxK = 32768;       // 1024 threads with 4 chunks each hold a row
 
-// The smallest workgroup that holds a row of K elements with at most 4 chunks a thread, one wave for short rows.
-#define DECX_RMSNORM_SHAPES(K, LAUNCH)       \
-    do {                                     \
-        if ((K) <= 512) LAUNCH(64, 1);       \
-        else if ((K) <= 1024) LAUNCH(128, 1); \
-        else if ((K) <= 2048) LAUNCH(256, 1); \
-        else if ((K) <= 4096) LAUNCH(256, 2); \
-        else if ((K) <= 8192) LAUNCH(256, 4); \
-        else if ((K) <= 16384) LAUNCH(512, 4); \
-        else LAUNCH(1024, 4);                \
+// The smallest workgroup that holds a row of K elements with at most MOST chunks a thread, one wave for short rows.  The
+// gradient holds three inputs twice, a row's and the next one's: 4 chunks in fp32 would leave registers for one workgroup a CU.
+#define DECX_RMSNORM_SHAPES(K, MOST, LAUNCH)               \
+    do {                                                   \
+        if ((K) <= 512) LAUNCH(64, 1);                     \
+        else if ((K) <= 1024) LAUNCH(128, 1);              \
+        else if ((K) <= 2048) LAUNCH(256, 1);              \
+        else if ((K) <= 4096) LAUNCH(256, 2);              \
+        else if ((K) <= 8192) LAUNCH(1024 / (MOST), MOST); \
+        else if ((K) <= 16384) LAUNCH(2048 / (MOST), MOST); \
+        else LAUNCH(1024, 4);                              \
     } while (0)
 
 template <int TYPE>
 static int rmsnorm_f8_launch(const RmsNormArgs& g) {
 #define DECX_LAUNCH(NT, CH) hipLaunchKernelGGL((rmsnorm_f8_kernel<TYPE, NT, CH>), dim3((unsigned)g.M), dim3(NT), 0, g_rt.stream, g)
-    DECX_RMSNORM_SHAPES(g.K, DECX_LAUNCH);
+    DECX_RMSNORM_SHAPES(g.K, 4, DECX_LAUNCH);
 #undef DECX_LAUNCH
     HIP_TRY(hipGetLastError());
     return 0;
 }
 template <int TYPE>
-static int rmsnorm_backward_launch(const RmsNormBackwardArgs& g, int groups) {
-#define DECX_LAUNCH(NT, CH) hipLaunchKernelGGL((rmsnorm_backward_kernel<TYPE, NT, CH>), dim3((unsigned)groups), dim3(NT), 0, g_rt.stream, g)
-    DECX_RMSNORM_SHAPES(g.K, DECX_LAUNCH);
+static int rmsnorm_backward_launch(const RmsNormBackwardArgs& g) {
+    const bool whole = g.K % 8 == 0;        // rows of whole chunks: no other way of loading beside theirs, which costs registers
+#define DECX_LAUNCH(NT, CH)                                                                                                    \
+    hipLaunchKernelGGL((whole ? rmsnorm_backward_kernel<TYPE, NT, CH, true> : rmsnorm_backward_kernel<TYPE, NT, CH, false>),       \
+                       dim3((unsigned)(g.row_groups + (g.dW ? cdiv(g.K, dw_columns(NT)) : 0))), dim3(NT), 0, g_rt.stream, g)
+    constexpr int MOST = TYPE == 0 ? 2 : 4;
+    DECX_RMSNORM_SHAPES(g.K, MOST, DECX_LAUNCH);
 #undef DECX_LAUNCH
     HIP_TRY(hipGetLastError());
     return 0;
@@ -326,15 +389,20 @@ int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float*
                     rmsnorm_backward_workspace(M, K));
     const int groups = rmsnorm_backward_groups(M, K, type == DECX_HIP_F32 ? 4 : 2);
     RmsNormBackwardArgs g = {};
-    g.H = H, g.W = W, g.dY = dY, g.dR = dR, g.rstd = rstd, g.dX = dX, g.partial = dW ? static_cast<float*>(work) : nullptr;
+    g.H = H, g.W = W, g.dY = dY, g.dR = dR, g.rstd = rstd, g.dX = dX, g.row_groups = groups;
+    // Few rows of inputs that the caches hold: the column workgroups (one launch: 200 x 1500 8.4 -> 5.6 us, 512 x 4096 10.7 ->
+    // 7.4, 512 x 8192 15.9 -> 13; 2048 x 512 would go 12.5 -> 29.8), unless dX overwrites what they read
+    const bool in_place = dX == H || dX == dY;
+    const bool columns = dW && !in_place && M <= 512 && (size_t)M * K <= (size_t)1 << 22;
+    if (columns) g.dW = dW;
+    else if (dW) g.partial = static_cast<float*>(work);
     g.ldh = (size_t)ldh, g.lddy = (size_t)lddy, g.lddr = (size_t)lddr, g.lddx = (size_t)lddx;
     g.M = M, g.K = K, g.rows_each = cdiv(M, groups);
     // 16-bit inputs of more than the memory-side cache's 256 MiB are read past the caches: 8192 x 8192, 402 MB, 104 us
     // against 112; 8192 x 1000, 49 MB, 36 against 31 (and in fp32, whose lanes read a line in two pieces, always slower)
     g.stream = (size_t)M * K * (dR ? 6 : 4) > ((size_t)256 << 20);
-    int rc = type == DECX_HIP_F32 ? rmsnorm_backward_launch<0>(g, groups)
-                                  : type == DECX_HIP_F16 ? rmsnorm_backward_launch<1>(g, groups) : rmsnorm_backward_launch<2>(g, groups);
-    if (rc || !dW) return rc;
+    int rc = type == DECX_HIP_F32 ? rmsnorm_backward_launch<0>(g) : type == DECX_HIP_F16 ? rmsnorm_backward_launch<1>(g) : rmsnorm_backward_launch<2>(g);
+    if (rc || !g.partial) return rc;
     if (K <= 2048)          // narrow pieces where wide ones would leave most of the chip idle
         hipLaunchKernelGGL(rmsnorm_dw_kernel<8>, dim3((unsigned)cdiv(K, 8)), dim3(256), 0, g_rt.stream, g.partial, groups, K, dW);
     else
