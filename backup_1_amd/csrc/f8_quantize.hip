@@ -12,7 +12,7 @@ namespace decx_hip {
 // 8-byte store.  A workgroup takes 16 rows x kQuantCols blocks, so that the scales of a block column leave as 64
 // consecutive bytes (one scale for a row and block lies `lds` elements from the row's next one).
 constexpr int kQuantCols = 4;
-template <int TYPE>
+template <int TYPE, bool WHOLE>
 __global__ __launch_bounds__(256) void f8_quantize_rows_kernel(const typename Wide<TYPE>::T* __restrict__ X, size_t ldx, int M, int K,
                                                                int e5m2, int e8m0, uint8_t* __restrict__ Q, size_t ldq,
                                                                void* __restrict__ S, size_t lds, int col_groups) {
@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void f8_quantize_rows_kernel(const typename Wi
 #pragma unroll
     for (int j = 0; j < kQuantCols; ++j) {
         const int k = (kb0 + j) * kScaleBlock + 8 * li;
-        x[j] = load8_part<TYPE>(X + row * ldx + (k < K ? k : 0), K - k, k);
+        x[j] = load8_part<TYPE, WHOLE>(X + row * ldx + (k < K ? k : 0), K - k, k);
     }
     const int blocks = (K + kScaleBlock - 1) / kScaleBlock;
 #pragma unroll
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void f8_quantize_rows_kernel(const typename Wi
 //   rows   : the scale of a row is a maximum over the 16 lanes of its group;
 //   columns: over the 8 rows of a thread, the 4 groups of a wave and, through LDS, the 4 waves;
 //   square : one maximum over the tile, the same codes in both orders.
-template <int TYPE, bool SQUARE>
+template <int TYPE, bool SQUARE, bool WHOLE>
 __global__ __launch_bounds__(256) void f8_quantize_tile_kernel(const typename Wide<TYPE>::T* __restrict__ X, size_t ldx, int M, int K,
                                                                int e5m2, int e8m0, uint8_t* __restrict__ Q, size_t ldq,
                                                                void* __restrict__ S, size_t lds, uint8_t* __restrict__ Qt, size_t ldqt,
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void f8_quantize_tile_kernel(const typename Wi
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const bool live = m0 + i < M;
-        x[i] = load8_part<TYPE>(X + (size_t)(live ? m0 + i : 0) * ldx + (k0 < K ? k0 : 0), live ? K - k0 : 0, k0);
+        x[i] = load8_part<TYPE, WHOLE>(X + (size_t)(live ? m0 + i : 0) * ldx + (k0 < K ? k0 : 0), live ? K - k0 : 0, k0);
     }
     BlockScale square;
     if (SQUARE) {
@@ -157,17 +157,19 @@ static int f8_quantize_launch(const void* X, int ldx, int M, int K, int block_ro
                               int lds, uint8_t* Qt, int ldqt, void* St, int ldst) {
     typedef typename Wide<TYPE>::T T;
     const T* x = static_cast<const T*>(X);
+    const bool whole = K % 8 == 0;               // rows of whole chunks (load_raw8_part)
     const int row_blocks = cdiv(M, kScaleBlock), col_blocks = cdiv(K, kScaleBlock);
     if (block_rows == 1 && !Qt) {
         const int col_groups = cdiv(col_blocks, kQuantCols);
         const long groups = (long)cdiv(M, 16) * col_groups;
         if (groups > 0x7fffffffL) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
-        hipLaunchKernelGGL(f8_quantize_rows_kernel<TYPE>, dim3((unsigned)groups), dim3(256), 0, g_rt.stream, x, (size_t)ldx, M, K, e5m2,
+        hipLaunchKernelGGL((whole ? f8_quantize_rows_kernel<TYPE, true> : f8_quantize_rows_kernel<TYPE, false>), dim3((unsigned)groups), dim3(256), 0, g_rt.stream, x, (size_t)ldx, M, K, e5m2,
                            e8m0, Q, (size_t)ldq, S, (size_t)lds, col_groups);
     } else {
         const long tiles = (long)row_blocks * col_blocks;
         if (tiles > 0x7fffffffL) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
-        auto kern = block_rows == 1 ? f8_quantize_tile_kernel<TYPE, false> : f8_quantize_tile_kernel<TYPE, true>;
+        auto kern = block_rows == 1 ? (whole ? f8_quantize_tile_kernel<TYPE, false, true> : f8_quantize_tile_kernel<TYPE, false, false>)
+                                    : (whole ? f8_quantize_tile_kernel<TYPE, true, true> : f8_quantize_tile_kernel<TYPE, true, false>);
         hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), 0, g_rt.stream, x, (size_t)ldx, M, K, e5m2, e8m0, Q, (size_t)ldq, S,
                            (size_t)lds, Qt, (size_t)ldqt, St, (size_t)ldst, col_blocks);
     }

@@ -46,29 +46,24 @@ struct RmsNormArgs {
     int M, K, e5m2, e8m0;
 };
 
-template <int TYPE, int NT, int CH>
+template <int TYPE, int NT, int CH, bool WHOLE>
 __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
     typedef typename Wide<TYPE>::T T;
     __shared__ float part[NT / kWave];
     const int K = g.K, m = xcd_row((int)blockIdx.x, g.M);
     const T* x = static_cast<const T*>(g.X) + (size_t)m * g.ldx;
     Eight h[CH];
-    auto load_sum = [&](auto whole_tag) {
-        constexpr bool WHOLE = decltype(whole_tag)::value;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            h[i] = load8_part<TYPE, WHOLE>(x + at, K - k, k);
-            if (g.R) {
-                const Eight r = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k, k);
-                // the sum is what the stream carries on, so it is rounded to its type here and the norm is taken of that
+    for (int i = 0; i < CH; ++i) {
+        const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+        h[i] = load8_part<TYPE, WHOLE>(x + at, K - k, k);
+        if (g.R) {
+            const Eight r = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k, k);
+            // the sum is what the stream carries on, so it is rounded to its type here and the norm is taken of that
 #pragma unroll
-                for (int e = 0; e < 8; ++e) h[i].v[e] = (float)(T)(h[i].v[e] + r.v[e]);
-            }
+            for (int e = 0; e < 8; ++e) h[i].v[e] = (float)(T)(h[i].v[e] + r.v[e]);
         }
-    };
-    if (K % 8 == 0) load_sum(std::true_type{});
-    else load_sum(std::false_type{});
+    }
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i)
@@ -87,7 +82,7 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-        const Eight w = load8_part<TYPE>(static_cast<const T*>(g.W) + at, K - k, k);
+        const Eight w = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.W) + at, K - k, k);
         Eight y;
 #pragma unroll
         for (int e = 0; e < 8; ++e) y.v[e] = TYPE == 0 ? h[i].v[e] * rstd * w.v[e] : h[i].v[e] * w.v[e] * rstd;     // 16-bit h * w is exact
@@ -313,7 +308,9 @@ constexpr int kRmsNormMaxK = 32768;       // 1024 threads with 4 chunks each hol
 
 template <int TYPE>
 static int rmsnorm_f8_launch(const RmsNormArgs& g) {
-#define DECX_LAUNCH(NT, CH) hipLaunchKernelGGL((rmsnorm_f8_kernel<TYPE, NT, CH>), dim3((unsigned)g.M), dim3(NT), 0, g_rt.stream, g)
+    const bool whole = g.K % 8 == 0;
+#define DECX_LAUNCH(NT, CH) \
+    hipLaunchKernelGGL((whole ? rmsnorm_f8_kernel<TYPE, NT, CH, true> : rmsnorm_f8_kernel<TYPE, NT, CH, false>), dim3((unsigned)g.M), dim3(NT), 0, g_rt.stream, g)
     DECX_RMSNORM_SHAPES(g.K, 4, DECX_LAUNCH);
 #undef DECX_LAUNCH
     HIP_TRY(hipGetLastError());
