@@ -6,6 +6,8 @@
 namespace decx_hip {
 
 constexpr int kScaleBlock = 128;      // elements along the contraction that share a scale
+constexpr int kMostExtent = 1 << 29;  // rows or columns of an operand: sums of sizes and 4-byte offsets of scales fit 32 bits
+constexpr long kMostThreads = 0xffffffffL;     // of a launch: the hardware counts them in 32 bits
 
 // Wide and vector types that may lie at any address: global memory takes such accesses on gfx950 as one instruction, so
 // rows whose pitch is no multiple of 16 bytes need no slower loader of their own.

@@ -162,12 +162,12 @@ static int f8_quantize_launch(const void* X, int ldx, int M, int K, int block_ro
     if (block_rows == 1 && !Qt) {
         const int col_groups = cdiv(col_blocks, kQuantCols);
         const long groups = (long)cdiv(M, 16) * col_groups;
-        if (groups > 0x7fffffffL) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
+        if (groups * 256 > kMostThreads) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
         hipLaunchKernelGGL((whole ? f8_quantize_rows_kernel<TYPE, true> : f8_quantize_rows_kernel<TYPE, false>), dim3((unsigned)groups), dim3(256), 0, g_rt.stream, x, (size_t)ldx, M, K, e5m2,
                            e8m0, Q, (size_t)ldq, S, (size_t)lds, col_groups);
     } else {
         const long tiles = (long)row_blocks * col_blocks;
-        if (tiles > 0x7fffffffL) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
+        if (tiles * 256 > kMostThreads) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
         auto kern = block_rows == 1 ? (whole ? f8_quantize_tile_kernel<TYPE, false, true> : f8_quantize_tile_kernel<TYPE, false, false>)
                                     : (whole ? f8_quantize_tile_kernel<TYPE, true, true> : f8_quantize_tile_kernel<TYPE, true, false>);
         hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), 0, g_rt.stream, x, (size_t)ldx, M, K, e5m2, e8m0, Q, (size_t)ldq, S,
@@ -183,6 +183,7 @@ int f8_quantize_enqueue(const void* X, int ldx, int type, int M, int K, int bloc
     if (!X || (!Q && !Qt)) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "null matrix pointer\n");
     if ((Q && !S) || (Qt && !St)) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "codes without their scales\n");
     if (M <= 0 || K <= 0) return fail(DECX_HIP_FAIL_DIMS, "Matrix Dims don't match each other");
+    if (M > kMostExtent || K > kMostExtent) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
     if (int rc = check_f8_codes(type, format, scale_type)) return rc;
     if (block_rows != 1 && block_rows != kScaleBlock) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "a block has 1 or 128 rows\n");
     const int row_scales = block_rows == 1 ? M : cdiv(M, kScaleBlock), col_scales = block_rows == 1 ? K : cdiv(K, kScaleBlock);

@@ -65,6 +65,7 @@ int f8gemm_enqueue(const uint8_t* A, int lda, int format_a, const void* SA, int 
     if (int rc = need_library_device()) return rc;
     if (!A || !B || !SA || !SB || !D) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "null matrix pointer\n");
     if (M <= 0 || N <= 0 || K <= 0) return fail(DECX_HIP_FAIL_DIMS, "Matrix Dims don't match each other");
+    if (M > kMostExtent || N > kMostExtent || K > kMostExtent) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
     if (int rc = check_f8_codes(type, format_a, scale_type)) return rc;
     if (int rc = check_f8_codes(type, format_b, scale_type)) return rc;
     if (b_block_rows != 1 && b_block_rows != kScaleBlock) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "a block has 1 or 128 rows\n");

@@ -308,6 +308,9 @@ constexpr int kRmsNormMaxK = 32768;       // 1024 threads with 4 chunks each hol
 
 template <int TYPE>
 static int rmsnorm_f8_launch(const RmsNormArgs& g) {
+    // a workgroup a row
+    if ((long)g.M * (g.K <= 512 ? 64 : g.K <= 1024 ? 128 : g.K <= 8192 ? 256 : g.K <= 16384 ? 512 : 1024) > kMostThreads)
+        return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
     const bool whole = g.K % 8 == 0;
 #define DECX_LAUNCH(NT, CH) \
     hipLaunchKernelGGL((whole ? rmsnorm_f8_kernel<TYPE, NT, CH, true> : rmsnorm_f8_kernel<TYPE, NT, CH, false>), dim3((unsigned)g.M), dim3(NT), 0, g_rt.stream, g)
@@ -336,6 +339,7 @@ int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const voi
     if (!H && !Y && !Q && !rstd) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "no result wanted\n");
     if (Q && !S) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "codes without their scales\n");
     if (M <= 0 || K <= 0) return fail(DECX_HIP_FAIL_DIMS, "Matrix Dims don't match each other");
+    if (M > kMostExtent) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
     if (K > kRmsNormMaxK) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "the norm takes rows of at most %d elements\n", kRmsNormMaxK);
     if (int rc = check_f8_codes(type, format, scale_type)) return rc;
     if (!(eps >= 0.f)) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "eps is negative or no number\n");
@@ -373,6 +377,7 @@ int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float*
     if (int rc = need_library_device()) return rc;
     if (!H || !W || !rstd || !dY || !dX) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "null matrix pointer\n");
     if (M <= 0 || K <= 0) return fail(DECX_HIP_FAIL_DIMS, "Matrix Dims don't match each other");
+    if (M > kMostExtent) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
     if (K > kRmsNormMaxK) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "the norm takes rows of at most %d elements\n", kRmsNormMaxK);
     if (int rc = check_f8_codes(type, DECX_HIP_E4M3, DECX_HIP_SCALE_F32)) return rc;
     if (ldh < K || lddy < K || (dR && lddr < K) || lddx < K)

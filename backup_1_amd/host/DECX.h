@@ -38,6 +38,8 @@ enum DECX_error_types {
 };
 // classes/store_types.h:24-28
 enum DATA_STORE_TYPE { Page_Locked = 0x00, Page_Default = 0x01 };
+// 8-bit formats of the products scaled by blocks (no counterpart in the reference): OCP e4m3 and e5m2
+enum f8_format { de_f8_e4m3 = 0, de_f8_e5m2 = 1 };
 // convolution/CUDA/conv_flags.h:16-20
 enum conv_property { de_conv_no_compensate = 0, de_conv_zero_compensate = 1 };
 }  // namespace decx
@@ -227,6 +229,28 @@ DH GEMM3(MatrixArray<float>& A, MatrixArray<float>& B, MatrixArray<float>& dst);
 DH GEMM3(MatrixArray<Half>& A, MatrixArray<Half>& B, MatrixArray<Half>& dst);
 DH GEMM3(MatrixArray<float>& A, MatrixArray<float>& B, MatrixArray<float>& C, MatrixArray<float>& dst);
 DH GEMM3(MatrixArray<Half>& A, MatrixArray<Half>& B, MatrixArray<Half>& C, MatrixArray<Half>& dst);
+// Products of 8-bit operands with a scale for each block of 128 along K (decx_hip_f8_quantize, decx_hip_f8gemm; the reference
+// has no 8-bit arithmetic, these stand beside its GEMM overloads).  A matrix (K wide, M high) is quantised to codes of its
+// size and scales (M / block_rows wide, K / 128 high, both rounded up; block_rows 1 or 128), fp32 or -- in a uchar matrix --
+// biased exponents of powers of two; Quantize_f8_T does the same of the transpose.  GEMM_f8 multiplies A (K wide, M high,
+// scaled by rows) with B, which holds one column of the product per row (K wide, N high) and is scaled by rows or by 128
+// rows, whichever its scales' width says: dst (N wide, M high) = A * B^T.
+DH Quantize_f8(GPU_Matrix<float>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int block_rows, const int format);
+DH Quantize_f8(GPU_Matrix<Half>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int block_rows, const int format);
+DH Quantize_f8(GPU_Matrix<float>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<uchar>& scales, const int block_rows, const int format);
+DH Quantize_f8(GPU_Matrix<Half>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<uchar>& scales, const int block_rows, const int format);
+DH Quantize_f8_T(GPU_Matrix<float>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int block_rows, const int format);
+DH Quantize_f8_T(GPU_Matrix<Half>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int block_rows, const int format);
+DH Quantize_f8_T(GPU_Matrix<float>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<uchar>& scales, const int block_rows, const int format);
+DH Quantize_f8_T(GPU_Matrix<Half>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<uchar>& scales, const int block_rows, const int format);
+DH GEMM_f8(GPU_Matrix<uchar>& A, GPU_Matrix<float>& scale_A, const int format_A, GPU_Matrix<uchar>& B, GPU_Matrix<float>& scale_B,
+           const int format_B, GPU_Matrix<float>& dst);
+DH GEMM_f8(GPU_Matrix<uchar>& A, GPU_Matrix<float>& scale_A, const int format_A, GPU_Matrix<uchar>& B, GPU_Matrix<float>& scale_B,
+           const int format_B, GPU_Matrix<Half>& dst);
+DH GEMM_f8(GPU_Matrix<uchar>& A, GPU_Matrix<uchar>& scale_A, const int format_A, GPU_Matrix<uchar>& B, GPU_Matrix<uchar>& scale_B,
+           const int format_B, GPU_Matrix<float>& dst);
+DH GEMM_f8(GPU_Matrix<uchar>& A, GPU_Matrix<uchar>& scale_A, const int format_A, GPU_Matrix<uchar>& B, GPU_Matrix<uchar>& scale_B,
+           const int format_B, GPU_Matrix<Half>& dst);
 // convolution/CUDA/im2col/conv2_mk_im2col.h:25.  flag: decx::conv_property.
 DH Conv2_MK_im2col(Tensor<float>& src, TensorArray<float>& kernel, Tensor<float>& dst, const int flag);
 // Device-resident flavour of the same convolution (the reference only has the host one; its GPU_Tensor /
@@ -248,6 +272,17 @@ namespace nn {
 DH ReLU_f(GPU_Matrix<float>& src, GPU_Matrix<float>& dst);
 DH ReLU_f_Rec(GPU_Matrix<float>& src, GPU_Matrix<float>& dst, GPU_Matrix<uchar>& rec_map);
 DH ReLU_f_Backward(GPU_Matrix<float>& src, GPU_Matrix<float>& dst, GPU_Matrix<uchar>& rec_map);
+// Root-mean-square norm of the rows of src + residual with its result as 8-bit codes scaled by rows (decx_hip_rmsnorm_f8), and
+// its gradient (decx_hip_rmsnorm_backward).  weight is one row; sum (which may be src or residual), codes, scales and rstd (one
+// row, a factor for each row of src) are sized as needed; grad_weight becomes one row.  dst may be grad.
+DH RMSNorm_f8(GPU_Matrix<float>& src, GPU_Matrix<float>& residual, GPU_Matrix<float>& weight, const float eps, GPU_Matrix<float>& sum,
+              GPU_Matrix<float>& rstd, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int format);
+DH RMSNorm_f8(GPU_Matrix<Half>& src, GPU_Matrix<Half>& residual, GPU_Matrix<Half>& weight, const float eps, GPU_Matrix<Half>& sum,
+              GPU_Matrix<float>& rstd, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int format);
+DH RMSNorm_f8_Backward(GPU_Matrix<float>& sum, GPU_Matrix<float>& weight, GPU_Matrix<float>& rstd, GPU_Matrix<float>& grad,
+                       GPU_Matrix<float>& dst, GPU_Matrix<float>& grad_weight);
+DH RMSNorm_f8_Backward(GPU_Matrix<Half>& sum, GPU_Matrix<Half>& weight, GPU_Matrix<float>& rstd, GPU_Matrix<Half>& grad,
+                       GPU_Matrix<Half>& dst, GPU_Matrix<float>& grad_weight);
 }  // namespace nn
 
 namespace cpu {

@@ -457,6 +457,154 @@ DH Conv2_MK_im2col(GPU_Tensor<Half>& src, GPU_TensorArray<Half>& kernel, GPU_Ten
 }
 }  // namespace cuda
 
+// ---- 8-bit products scaled by blocks of 128 (decx_hip_f8_quantize, decx_hip_f8gemm, decx_hip_rmsnorm_f8) ---------------------
+namespace {
+template <typename T> struct F8Wide;
+template <> struct F8Wide<float> { static constexpr int type = DECX_HIP_F32; };
+template <> struct F8Wide<Half> { static constexpr int type = DECX_HIP_F16; };
+template <typename S> struct F8Scale;
+template <> struct F8Scale<float> { static constexpr int type = DECX_HIP_SCALE_F32; };
+template <> struct F8Scale<uchar> { static constexpr int type = DECX_HIP_SCALE_E8M0; };
+
+uint blocks_of_128(uint n) { return (n + 127) / 128; }
+
+// sizes an output matrix; a success has error_type DECX_SUCCESS
+template <typename T>
+DH size_output(decx::_GPU_Matrix<T>* m, uint w, uint h) {
+    if (m->re_construct(w, h)) return ok();
+    return m->last_status == DECX_HIP_FAIL_ALLOCATION ? alloc_fail() : from_status(m->last_status);
+}
+
+template <typename T, typename S>
+DH quantize_f8(GPU_Matrix<T>& src_, GPU_Matrix<uchar>& codes_, GPU_Matrix<S>& scales_, int block_rows, int format, bool transpose) {
+    auto* src = dynamic_cast<decx::_GPU_Matrix<T>*>(&src_);
+    auto* codes = dynamic_cast<decx::_GPU_Matrix<uchar>*>(&codes_);
+    auto* scales = dynamic_cast<decx::_GPU_Matrix<S>*>(&scales_);
+    if (!src || !codes || !scales || static_cast<void*>(codes) == static_cast<void*>(scales)) return DH{decx::DECX_FAIL_ErrorParams, kNotFactory};
+    if (!decx_hip_is_init()) return not_init();
+    if (!src->Mat.ptr || !src->width || !src->height) return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
+    const uint rows = transpose ? src->width : src->height, cols = transpose ? src->height : src->width;
+    DH status = size_output(codes, cols, rows);
+    if (status.error_type == decx::DECX_SUCCESS) status = size_output(scales, block_rows == 128 ? blocks_of_128(rows) : rows, blocks_of_128(cols));
+    if (status.error_type != decx::DECX_SUCCESS) return status;
+    uint8_t* q = codes->Mat.ptr;
+    const int ldq = (int)codes->pitch, lds = (int)scales->pitch;
+    return from_status(decx_hip_f8_quantize(src->Mat.ptr, (int)src->pitch, F8Wide<T>::type, (int)src->height, (int)src->width, block_rows, format,
+                                            F8Scale<S>::type, transpose ? nullptr : q, ldq, transpose ? nullptr : scales->Mat.ptr, lds,
+                                            transpose ? q : nullptr, ldq, transpose ? scales->Mat.ptr : nullptr, lds));
+}
+
+template <typename T, typename S>
+DH gemm_f8(GPU_Matrix<uchar>& A_, GPU_Matrix<S>& sA_, int fA, GPU_Matrix<uchar>& B_, GPU_Matrix<S>& sB_, int fB, GPU_Matrix<T>& dst_) {
+    auto* A = dynamic_cast<decx::_GPU_Matrix<uchar>*>(&A_);
+    auto* B = dynamic_cast<decx::_GPU_Matrix<uchar>*>(&B_);
+    auto* sA = dynamic_cast<decx::_GPU_Matrix<S>*>(&sA_);
+    auto* sB = dynamic_cast<decx::_GPU_Matrix<S>*>(&sB_);
+    auto* dst = dynamic_cast<decx::_GPU_Matrix<T>*>(&dst_);
+    if (!A || !B || !sA || !sB || !dst) return DH{decx::DECX_FAIL_ErrorParams, kNotFactory};
+    if (!decx_hip_is_init()) return not_init();
+    const uint M = A->height, N = B->height, K = A->width;
+    if (!A->Mat.ptr || !B->Mat.ptr || !sA->Mat.ptr || !sB->Mat.ptr || !M || !N || !K) return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
+    const bool by_rows = sB->width == N, by_blocks = sB->width == blocks_of_128(N);
+    if (B->width != K || sA->width != M || sA->height != blocks_of_128(K) || sB->height != blocks_of_128(K) || !(by_rows || by_blocks))
+        return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
+    const DH status = size_output(dst, N, M);
+    if (status.error_type != decx::DECX_SUCCESS) return status;
+    return from_status(decx_hip_f8gemm(A->Mat.ptr, (int)A->pitch, fA, sA->Mat.ptr, (int)sA->pitch, B->Mat.ptr, (int)B->pitch, fB, sB->Mat.ptr,
+                                       (int)sB->pitch, by_rows ? 1 : 128, F8Scale<S>::type, nullptr, 0, dst->Mat.ptr, (int)dst->pitch,
+                                       F8Wide<T>::type, (int)M, (int)N, (int)K));
+}
+
+template <typename T>
+DH rmsnorm_f8(GPU_Matrix<T>& src_, GPU_Matrix<T>& residual_, GPU_Matrix<T>& weight_, float eps, GPU_Matrix<T>& sum_, GPU_Matrix<float>& rstd_,
+              GPU_Matrix<uchar>& codes_, GPU_Matrix<float>& scales_, int format) {
+    auto* src = dynamic_cast<decx::_GPU_Matrix<T>*>(&src_);
+    auto* residual = dynamic_cast<decx::_GPU_Matrix<T>*>(&residual_);
+    auto* weight = dynamic_cast<decx::_GPU_Matrix<T>*>(&weight_);
+    auto* sum = dynamic_cast<decx::_GPU_Matrix<T>*>(&sum_);
+    auto* rstd = dynamic_cast<decx::_GPU_Matrix<float>*>(&rstd_);
+    auto* codes = dynamic_cast<decx::_GPU_Matrix<uchar>*>(&codes_);
+    auto* scales = dynamic_cast<decx::_GPU_Matrix<float>*>(&scales_);
+    if (!src || !residual || !weight || !sum || !rstd || !codes || !scales || rstd == scales) return DH{decx::DECX_FAIL_ErrorParams, kNotFactory};
+    if (!decx_hip_is_init()) return not_init();
+    const uint M = src->height, K = src->width;
+    if (!src->Mat.ptr || !residual->Mat.ptr || !weight->Mat.ptr || !M || !K || residual->width != K || residual->height != M || weight->width != K)
+        return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
+    DH status = size_output(sum, K, M);
+    if (status.error_type == decx::DECX_SUCCESS) status = size_output(rstd, M, 1);
+    if (status.error_type == decx::DECX_SUCCESS) status = size_output(codes, K, M);
+    if (status.error_type == decx::DECX_SUCCESS) status = size_output(scales, M, blocks_of_128(K));
+    if (status.error_type != decx::DECX_SUCCESS) return status;
+    return from_status(decx_hip_rmsnorm_f8(src->Mat.ptr, (int)src->pitch, residual->Mat.ptr, (int)residual->pitch, weight->Mat.ptr, eps,
+                                           F8Wide<T>::type, (int)M, (int)K, sum->Mat.ptr, (int)sum->pitch, rstd->Mat.ptr, nullptr, 0,
+                                           codes->Mat.ptr, (int)codes->pitch, scales->Mat.ptr, (int)scales->pitch, format, DECX_HIP_SCALE_F32));
+}
+
+template <typename T>
+DH rmsnorm_f8_backward(GPU_Matrix<T>& sum_, GPU_Matrix<T>& weight_, GPU_Matrix<float>& rstd_, GPU_Matrix<T>& grad_, GPU_Matrix<T>& dst_,
+                       GPU_Matrix<float>& grad_weight_) {
+    auto* sum = dynamic_cast<decx::_GPU_Matrix<T>*>(&sum_);
+    auto* weight = dynamic_cast<decx::_GPU_Matrix<T>*>(&weight_);
+    auto* rstd = dynamic_cast<decx::_GPU_Matrix<float>*>(&rstd_);
+    auto* grad = dynamic_cast<decx::_GPU_Matrix<T>*>(&grad_);
+    auto* dst = dynamic_cast<decx::_GPU_Matrix<T>*>(&dst_);
+    auto* grad_weight = dynamic_cast<decx::_GPU_Matrix<float>*>(&grad_weight_);
+    if (!sum || !weight || !rstd || !grad || !dst || !grad_weight || rstd == grad_weight || rstd->shares_block_with(*grad_weight))
+        return DH{decx::DECX_FAIL_ErrorParams, kNotFactory};
+    if (!decx_hip_is_init()) return not_init();
+    const uint M = sum->height, K = sum->width;
+    if (!sum->Mat.ptr || !weight->Mat.ptr || !rstd->Mat.ptr || !grad->Mat.ptr || !M || !K || weight->width != K || rstd->width != M ||
+        grad->width != K || grad->height != M)
+        return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
+    DH status = size_output(dst, K, M);
+    if (status.error_type == decx::DECX_SUCCESS) status = size_output(grad_weight, K, 1);
+    if (status.error_type != decx::DECX_SUCCESS) return status;
+    DeviceTemp work;
+    const size_t bytes = decx_hip_rmsnorm_backward_workspace((int)M, (int)K);
+    if (int rc = work.alloc(bytes)) return rc == DECX_HIP_FAIL_ALLOCATION ? alloc_fail() : from_status(rc);
+    return from_status(decx_hip_rmsnorm_backward(sum->Mat.ptr, (int)sum->pitch, weight->Mat.ptr, rstd->Mat.ptr, grad->Mat.ptr, (int)grad->pitch,
+                                                 nullptr, 0, F8Wide<T>::type, (int)M, (int)K, dst->Mat.ptr, (int)dst->pitch,
+                                                 grad_weight->Mat.ptr, work.ptr, bytes));
+}
+}  // namespace
+
+namespace cuda {
+#define DECX_QUANTIZE_F8(T, S)                                                                                                               \
+    DH Quantize_f8(GPU_Matrix<T>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<S>& scales, const int block_rows, const int format) {           \
+        return quantize_f8<T, S>(src, codes, scales, block_rows, format, false);                                                            \
+    }                                                                                                                                       \
+    DH Quantize_f8_T(GPU_Matrix<T>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<S>& scales, const int block_rows, const int format) {         \
+        return quantize_f8<T, S>(src, codes, scales, block_rows, format, true);                                                             \
+    }                                                                                                                                       \
+    DH GEMM_f8(GPU_Matrix<uchar>& A, GPU_Matrix<S>& scale_A, const int format_A, GPU_Matrix<uchar>& B, GPU_Matrix<S>& scale_B,              \
+               const int format_B, GPU_Matrix<T>& dst) {                                                                                    \
+        return gemm_f8<T, S>(A, scale_A, format_A, B, scale_B, format_B, dst);                                                              \
+    }
+DECX_QUANTIZE_F8(float, float)
+DECX_QUANTIZE_F8(float, uchar)
+DECX_QUANTIZE_F8(Half, float)
+DECX_QUANTIZE_F8(Half, uchar)
+}  // namespace cuda
+
+namespace nn {
+DH RMSNorm_f8(GPU_Matrix<float>& src, GPU_Matrix<float>& residual, GPU_Matrix<float>& weight, const float eps, GPU_Matrix<float>& sum,
+              GPU_Matrix<float>& rstd, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int format) {
+    return rmsnorm_f8<float>(src, residual, weight, eps, sum, rstd, codes, scales, format);
+}
+DH RMSNorm_f8(GPU_Matrix<Half>& src, GPU_Matrix<Half>& residual, GPU_Matrix<Half>& weight, const float eps, GPU_Matrix<Half>& sum,
+              GPU_Matrix<float>& rstd, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int format) {
+    return rmsnorm_f8<Half>(src, residual, weight, eps, sum, rstd, codes, scales, format);
+}
+DH RMSNorm_f8_Backward(GPU_Matrix<float>& sum, GPU_Matrix<float>& weight, GPU_Matrix<float>& rstd, GPU_Matrix<float>& grad,
+                       GPU_Matrix<float>& dst, GPU_Matrix<float>& grad_weight) {
+    return rmsnorm_f8_backward<float>(sum, weight, rstd, grad, dst, grad_weight);
+}
+DH RMSNorm_f8_Backward(GPU_Matrix<Half>& sum, GPU_Matrix<Half>& weight, GPU_Matrix<float>& rstd, GPU_Matrix<Half>& grad,
+                       GPU_Matrix<Half>& dst, GPU_Matrix<float>& grad_weight) {
+    return rmsnorm_f8_backward<Half>(sum, weight, rstd, grad, dst, grad_weight);
+}
+}  // namespace nn
+
 // ---- nn::ReLU (nn/operators/ReLU.h:169-210) ----------------------------------------------------------------------
 namespace nn {
 namespace {
