@@ -763,6 +763,12 @@ int decx_hip_f8_call(int call, const int64_t* a, int blocking) {
     auto bytes = [&](int i) { return static_cast<uint8_t*>(ptr(i)); };
     auto floats = [&](int i) { return static_cast<float*>(ptr(i)); };
     auto num = [&](int i) { return (int)a[i]; };
+    // which of a call's arguments are int: a value beyond that is refused, not cut
+    static const unsigned ints[4] = {0xaafeu /* 1-7, 9, 11, 13, 15 */, 0xfaed6u /* 1, 2, 4, 6, 7, 9-11, 13, 15-19 */,
+                                     0xea5cau /* 1, 3, 6-8, 10, 13, 15, 17-19 */, 0x17a2u /* 1, 5, 7-10, 12 */};
+    if (call >= 0 && call < 4)
+        for (int i = 0; i < 20; ++i)
+            if ((ints[call] >> i & 1u) && a[i] != (int64_t)num(i)) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "argument %d is no int\n", i);
     int rc;
     switch (call) {
         case DECX_HIP_CALL_F8_QUANTIZE:

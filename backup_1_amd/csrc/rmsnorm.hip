@@ -85,7 +85,7 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
         const Eight w = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.W) + at, K - k, k);
         Eight y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y.v[e] = TYPE == 0 ? h[i].v[e] * rstd * w.v[e] : h[i].v[e] * w.v[e] * rstd;     // 16-bit h * w is exact
+        for (int e = 0; e < 8; ++e) y.v[e] = h[i].v[e] * rstd * w.v[e];     // in this order: |h * rstd| <= sqrt(K), h * w may overflow
         if (g.Y) store8_part<TYPE>(static_cast<T*>(g.Y) + (size_t)m * g.ldy + at, y, K - k);
         if (g.Q) {
             // the codes are rounded from fp32, not from y's own type; elements past K are zeros

@@ -256,3 +256,24 @@ def test_refusals(gpu):
         refused(0x0d, **{n: 63})
     refused(0x0d, dW=at[6] + 2)
     refused(0x0d, dX=at[5] + 1)
+
+
+def test_weights_whose_product_with_the_row_overflows(gpu):
+    x = ref.to_type(workloads.normal((5, 200), 40).astype(np.float32) * np.float32(2.0 ** 60), capi.BF16)
+    w = ref.to_type(workloads.normal((1, 200), 41).astype(np.float32) * np.float32(2.0 ** 80), capi.BF16)      # h * w beyond 2^128, y is not
+    check(x, None, w, capi.BF16, run(x, None, w, capi.BF16))
+
+
+@pytest.mark.parametrize("call", ["quantize", "f8gemm", "norm", "backward"])
+def test_integers_beyond_an_int_are_refused(gpu, call):
+    d, far = capi.DeviceBuffer(64), 1 << 32
+    with pytest.raises(capi.DecxHipError) as e:
+        if call == "quantize":
+            capi.f8_quantize(d.ptr, 16, 0, 1, far + 1, 1, 0, 0, d.ptr, 16, d.ptr, 1)
+        elif call == "f8gemm":
+            capi.f8gemm(d.ptr, 16, 0, d.ptr, 1, d.ptr, 16, 0, d.ptr, 1, 128, 0, d.ptr, 1, 0, 1, 1, far + 1)
+        elif call == "norm":
+            capi.rmsnorm_f8(d.ptr, far + 16, None, 0, d.ptr, 1e-5, 0, 1, 1, d.ptr, 16, None, None, 0, None, 0, None, 0)
+        else:
+            capi.rmsnorm_backward(d.ptr, 16, d.ptr, d.ptr, d.ptr, 16, None, 0, 0, 1, 1, d.ptr, far + 16, None, None, 0)
+    assert e.value.code == 0x0d and "no int" in str(e.value)
