@@ -21,11 +21,18 @@ __global__ __launch_bounds__(256) void f8_quantize_rows_kernel(const typename Wi
     const int kb0 = (int)(blockIdx.x % (unsigned)col_groups) * kQuantCols;
     const int rows = M;
     const size_t row = (size_t)(m < rows ? m : rows - 1);
+    RawEight<TYPE> raw[kQuantCols];
     Eight x[kQuantCols];
 #pragma unroll
     for (int j = 0; j < kQuantCols; ++j) {
         const int k = (kb0 + j) * kScaleBlock + 8 * li;
-        x[j] = load8_part<TYPE, WHOLE>(X + row * ldx + (k < K ? k : 0), K - k, k);
+        raw[j] = fetch8_part<TYPE, false, WHOLE>(X + row * ldx + (k < K ? k : 0), K - k, k);
+    }
+#pragma unroll
+    for (int j = 0; j < kQuantCols; ++j) {
+        const int k = (kb0 + j) * kScaleBlock + 8 * li;
+        settle8_part<TYPE, WHOLE>(raw[j], K - k, k);
+        x[j] = widen8<TYPE>(raw[j]);
     }
     const int blocks = (K + kScaleBlock - 1) / kScaleBlock;
 #pragma unroll
@@ -56,11 +63,17 @@ __global__ __launch_bounds__(256) void f8_quantize_tile_kernel(const typename Wi
     const int tid = threadIdx.x, rg = tid >> 4, c = tid & 15, wave = tid >> 6;
     const int mb = (int)(blockIdx.x / (unsigned)col_blocks), kb = (int)(blockIdx.x % (unsigned)col_blocks);
     const int m0 = mb * kScaleBlock + 8 * rg, k0 = kb * kScaleBlock + 8 * c;
+    RawEight<TYPE> raw[8];
     Eight x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const bool live = m0 + i < M;
-        x[i] = load8_part<TYPE, WHOLE>(X + (size_t)(live ? m0 + i : 0) * ldx + (k0 < K ? k0 : 0), live ? K - k0 : 0, k0);
+        raw[i] = fetch8_part<TYPE, false, WHOLE>(X + (size_t)(live ? m0 + i : 0) * ldx + (k0 < K ? k0 : 0), live ? K - k0 : 0, k0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        settle8_part<TYPE, WHOLE>(raw[i], K - k0, k0);          // rows past the last are zeros either way
+        x[i] = widen8<TYPE>(raw[i]);
     }
     BlockScale square;
     if (SQUARE) {
@@ -157,7 +170,7 @@ static int f8_quantize_launch(const void* X, int ldx, int M, int K, int block_ro
                               int lds, uint8_t* Qt, int ldqt, void* St, int ldst) {
     typedef typename Wide<TYPE>::T T;
     const T* x = static_cast<const T*>(X);
-    const bool whole = K % 8 == 0;               // rows of whole chunks (load_raw8_part)
+    const bool whole = K % 8 == 0;               // rows of whole chunks (fetch8_part)
     const int row_blocks = cdiv(M, kScaleBlock), col_blocks = cdiv(K, kScaleBlock);
     if (block_rows == 1 && !Qt) {
         const int col_groups = cdiv(col_blocks, kQuantCols);

@@ -53,12 +53,21 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
     const int K = g.K, m = xcd_row((int)blockIdx.x, g.M);
     const T* x = static_cast<const T*>(g.X) + (size_t)m * g.ldx;
     Eight h[CH];
+    RawEight<TYPE> raw_x[CH], raw_r[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-        h[i] = load8_part<TYPE, WHOLE>(x + at, K - k, k);
+        raw_x[i] = fetch8_part<TYPE, false, WHOLE>(x + at, K - k, k);
+        if (g.R) raw_r[i] = fetch8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k, k);
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int k = 8 * ((int)threadIdx.x + i * NT);
+        settle8_part<TYPE, WHOLE>(raw_x[i], K - k, k);
+        h[i] = widen8<TYPE>(raw_x[i]);
         if (g.R) {
-            const Eight r = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k, k);
+            settle8_part<TYPE, WHOLE>(raw_r[i], K - k, k);
+            const Eight r = widen8<TYPE>(raw_r[i]);
             // the sum is what the stream carries on, so it is rounded to its type here and the norm is taken of that
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[i].v[e] = (float)(T)(h[i].v[e] + r.v[e]);
@@ -133,11 +142,13 @@ __device__ __forceinline__ void rmsnorm_dw_columns(const RmsNormBackwardArgs& g,
         for (int j = 0; j < AHEAD; ++j) {
             const int m = m0 + GROUPS * j, row = m < g.M ? m : 0;
             rstd[j] = m < g.M ? g.rstd[row] : 0.f;
-            h[j] = load_raw8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.H) + (size_t)row * g.ldh + at, m < g.M ? g.K - k : 0, k);
-            dy[j] = load_raw8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.dY) + (size_t)row * g.lddy + at, m < g.M ? g.K - k : 0, k);
+            h[j] = fetch8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.H) + (size_t)row * g.ldh + at, m < g.M ? g.K - k : 0, k);
+            dy[j] = fetch8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.dY) + (size_t)row * g.lddy + at, m < g.M ? g.K - k : 0, k);
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
+            settle8_part<TYPE, WHOLE>(h[j], g.K - k, k);            // rows past the last are zeros either way
+            settle8_part<TYPE, WHOLE>(dy[j], g.K - k, k);
             const Eight hv = widen8<TYPE>(h[j]), yv = widen8<TYPE>(dy[j]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] = __builtin_fmaf(yv.v[e], hv.v[e] * rstd[j], sum[e]);
@@ -188,9 +199,9 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            r.h[i] = load_raw8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k, k);
-            r.dy[i] = load_raw8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k, k);
-            if (g.dR) r.dr[i] = load_raw8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k, k);
+            r.h[i] = fetch8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k, k);
+            r.dy[i] = fetch8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k, k);
+            if (g.dR) r.dr[i] = fetch8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k, k);
         }
     };
     auto load_row = [&](Row& r, int m) {
@@ -200,7 +211,7 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
     Row next;
     load_row(next, first);
     for (int m = first; m < last; ++m) {
-        const Row row = next;
+        Row row = next;
         if (m + 1 < last) load_row(next, m + 1);
         const float rstd = row.rstd;
         Eight n[CH], dn[CH];                                    // n and g
@@ -209,6 +220,8 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
             const Eight w = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.W) + at, K - k, k);
+            settle8_part<TYPE, WHOLE>(row.h[i], K - k, k);
+            settle8_part<TYPE, WHOLE>(row.dy[i], K - k, k);
             n[i] = widen8<TYPE>(row.h[i]);
             dn[i] = widen8<TYPE>(row.dy[i]);
 #pragma unroll
@@ -228,6 +241,7 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
 #pragma unroll
             for (int e = 0; e < 8; ++e) dx.v[e] = rstd * __builtin_fmaf(-n[i].v[e], mean, dn[i].v[e]);
             if (g.dR) {
+                settle8_part<TYPE, WHOLE>(row.dr[i], K - k, k);
                 const Eight dr = widen8<TYPE>(row.dr[i]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dx.v[e] += dr.v[e];
