@@ -51,27 +51,30 @@ __device__ __forceinline__ u32x4 bytes_down(u32x4 v, int n) {
     if (n > 0) lo = lo >> (8 * n) | hi << (64 - 8 * n), hi >>= 8 * n;
     return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
-// The first `n` of 8 elements of a row (n may be <= 0 or > 8), the others 0, in two parts; `at` elements of the row lie before
-// them.  Reads nothing beyond the n: what is left of a row is fetched as the row's last 8 elements, one load instead of n.
-// fetch8_part issues the load and settle8_part moves the elements down, so that loads may stay in flight in between (moving
-// them at once, a wave with a row's end waited before its next load: norm's gradient of 4096 x 4095 bf16 took 49 us, now 41; 4096 x
-// 4096 29).  WHOLE: n is at least 8 or at most 0 (the row's length is a multiple of 8), which saves the moving's registers.
-template <int TYPE, bool STREAM = false, bool WHOLE = false>
-__device__ __forceinline__ RawEight<TYPE> fetch8_part(const typename Wide<TYPE>::T* p, int n, int at) {
+// The first `n` of 8 elements of a row (n may be <= 0 or > 8), the others 0, in two parts.  Reads nothing beyond the n: what
+// is left of a row is fetched as the row's last 8 elements, one load instead of n.  fetch8_part issues the load, settle8_part
+// moves the elements down, so that loads may stay in flight in between (moved at once, a wave with a row's end waited before
+// its next load: norm's gradient of 4096 x 4095 bf16 took 49 us, now 41).  ROWS says what the kernel's rows are like: shorter
+// than 8 elements, of any greater length, or of a multiple of 8 (nothing to move, fewer registers); short rows have kernels of
+// their own because their loads one by one, never taken, still cost the others (gradient of 4096 x 8190 bf16 82 -> 77 us).
+enum { kRowsShort = 0, kRowsRagged = 1, kRowsWhole = 2 };
+inline int rows_kind(int K) { return K % 8 == 0 ? kRowsWhole : K > 8 ? kRowsRagged : kRowsShort; }
+template <int TYPE, int ROWS, bool STREAM = false>
+__device__ __forceinline__ RawEight<TYPE> fetch8_part(const typename Wide<TYPE>::T* p, int n) {
     RawEight<TYPE> r = {};
     if (n <= 0) return r;
-    if (WHOLE || n >= 8 || at >= 8) return load_raw8<TYPE, STREAM>(WHOLE || n >= 8 ? p : p + (n - 8));
+    if constexpr (ROWS != kRowsShort) return load_raw8<TYPE, STREAM>(ROWS == kRowsWhole || n >= 8 ? p : p + (n - 8));
 #pragma unroll
-    for (int e = 0; e < 8; ++e)                                 // a row shorter than 8
+    for (int e = 0; e < 8; ++e)
         if (e < n) {
             if constexpr (TYPE == 0) r.w[e >> 2][e & 3] = reinterpret_cast<const uint32_t*>(p)[e];
             else r.w[0][e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
         }
     return r;
 }
-template <int TYPE, bool WHOLE = false>
-__device__ __forceinline__ void settle8_part(RawEight<TYPE>& r, int n, int at) {
-    if (WHOLE || n >= 8 || n <= 0 || at < 8) return;
+template <int TYPE, int ROWS>
+__device__ __forceinline__ void settle8_part(RawEight<TYPE>& r, int n) {
+    if (ROWS != kRowsRagged || n >= 8 || n <= 0) return;
     if constexpr (TYPE == 0) {
         uint32_t w[8];
 #pragma unroll
@@ -102,10 +105,10 @@ __device__ __forceinline__ Eight widen8(const RawEight<TYPE>& raw) {
     }
     return r;
 }
-template <int TYPE, bool WHOLE = false>
-__device__ __forceinline__ Eight load8_part(const typename Wide<TYPE>::T* p, int n, int at) {
-    RawEight<TYPE> r = fetch8_part<TYPE, false, WHOLE>(p, n, at);
-    settle8_part<TYPE, WHOLE>(r, n, at);
+template <int TYPE, int ROWS>
+__device__ __forceinline__ Eight load8_part(const typename Wide<TYPE>::T* p, int n) {
+    RawEight<TYPE> r = fetch8_part<TYPE, ROWS>(p, n);
+    settle8_part<TYPE, ROWS>(r, n);
     return widen8<TYPE>(r);
 }
 // rounds to nearest even, once

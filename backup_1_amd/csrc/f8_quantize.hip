@@ -12,7 +12,7 @@ namespace decx_hip {
 // 8-byte store.  A workgroup takes 16 rows x kQuantCols blocks, so that the scales of a block column leave as 64
 // consecutive bytes (one scale for a row and block lies `lds` elements from the row's next one).
 constexpr int kQuantCols = 4;
-template <int TYPE, bool WHOLE>
+template <int TYPE, int ROWS>
 __global__ __launch_bounds__(256) void f8_quantize_rows_kernel(const typename Wide<TYPE>::T* __restrict__ X, size_t ldx, int M, int K,
                                                                int e5m2, int e8m0, uint8_t* __restrict__ Q, size_t ldq,
                                                                void* __restrict__ S, size_t lds, int col_groups) {
@@ -26,12 +26,12 @@ __global__ __launch_bounds__(256) void f8_quantize_rows_kernel(const typename Wi
 #pragma unroll
     for (int j = 0; j < kQuantCols; ++j) {
         const int k = (kb0 + j) * kScaleBlock + 8 * li;
-        raw[j] = fetch8_part<TYPE, false, WHOLE>(X + row * ldx + (k < K ? k : 0), K - k, k);
+        raw[j] = fetch8_part<TYPE, ROWS>(X + row * ldx + (k < K ? k : 0), K - k);
     }
 #pragma unroll
     for (int j = 0; j < kQuantCols; ++j) {
         const int k = (kb0 + j) * kScaleBlock + 8 * li;
-        settle8_part<TYPE, WHOLE>(raw[j], K - k, k);
+        settle8_part<TYPE, ROWS>(raw[j], K - k);
         x[j] = widen8<TYPE>(raw[j]);
     }
     const int blocks = (K + kScaleBlock - 1) / kScaleBlock;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void f8_quantize_rows_kernel(const typename Wi
 //   rows   : the scale of a row is a maximum over the 16 lanes of its group;
 //   columns: over the 8 rows of a thread, the 4 groups of a wave and, through LDS, the 4 waves;
 //   square : one maximum over the tile, the same codes in both orders.
-template <int TYPE, bool SQUARE, bool WHOLE>
+template <int TYPE, bool SQUARE, int ROWS>
 __global__ __launch_bounds__(256) void f8_quantize_tile_kernel(const typename Wide<TYPE>::T* __restrict__ X, size_t ldx, int M, int K,
                                                                int e5m2, int e8m0, uint8_t* __restrict__ Q, size_t ldq,
                                                                void* __restrict__ S, size_t lds, uint8_t* __restrict__ Qt, size_t ldqt,
@@ -68,11 +68,11 @@ __global__ __launch_bounds__(256) void f8_quantize_tile_kernel(const typename Wi
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const bool live = m0 + i < M;
-        raw[i] = fetch8_part<TYPE, false, WHOLE>(X + (size_t)(live ? m0 + i : 0) * ldx + (k0 < K ? k0 : 0), live ? K - k0 : 0, k0);
+        raw[i] = fetch8_part<TYPE, ROWS>(X + (size_t)(live ? m0 + i : 0) * ldx + (k0 < K ? k0 : 0), live ? K - k0 : 0);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        settle8_part<TYPE, WHOLE>(raw[i], K - k0, k0);          // rows past the last are zeros either way
+        settle8_part<TYPE, ROWS>(raw[i], K - k0);          // rows past the last are zeros either way
         x[i] = widen8<TYPE>(raw[i]);
     }
     BlockScale square;
@@ -170,19 +170,27 @@ static int f8_quantize_launch(const void* X, int ldx, int M, int K, int block_ro
                               int lds, uint8_t* Qt, int ldqt, void* St, int ldst) {
     typedef typename Wide<TYPE>::T T;
     const T* x = static_cast<const T*>(X);
-    const bool whole = K % 8 == 0;               // rows of whole chunks (fetch8_part)
+    const int rows = rows_kind(K);
     const int row_blocks = cdiv(M, kScaleBlock), col_blocks = cdiv(K, kScaleBlock);
     if (block_rows == 1 && !Qt) {
         const int col_groups = cdiv(col_blocks, kQuantCols);
         const long groups = (long)cdiv(M, 16) * col_groups;
         if (groups * 256 > kMostThreads) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
-        hipLaunchKernelGGL((whole ? f8_quantize_rows_kernel<TYPE, true> : f8_quantize_rows_kernel<TYPE, false>), dim3((unsigned)groups), dim3(256), 0, g_rt.stream, x, (size_t)ldx, M, K, e5m2,
-                           e8m0, Q, (size_t)ldq, S, (size_t)lds, col_groups);
+        auto kern = rows == kRowsWhole    ? f8_quantize_rows_kernel<TYPE, kRowsWhole>
+                    : rows == kRowsRagged ? f8_quantize_rows_kernel<TYPE, kRowsRagged>
+                                          : f8_quantize_rows_kernel<TYPE, kRowsShort>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, g_rt.stream, x, (size_t)ldx, M, K, e5m2, e8m0, Q, (size_t)ldq, S, (size_t)lds,
+                           col_groups);
     } else {
         const long tiles = (long)row_blocks * col_blocks;
         if (tiles * 256 > kMostThreads) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
-        auto kern = block_rows == 1 ? (whole ? f8_quantize_tile_kernel<TYPE, false, true> : f8_quantize_tile_kernel<TYPE, false, false>)
-                                    : (whole ? f8_quantize_tile_kernel<TYPE, true, true> : f8_quantize_tile_kernel<TYPE, true, false>);
+        auto square = rows == kRowsWhole    ? f8_quantize_tile_kernel<TYPE, true, kRowsWhole>
+                      : rows == kRowsRagged ? f8_quantize_tile_kernel<TYPE, true, kRowsRagged>
+                                            : f8_quantize_tile_kernel<TYPE, true, kRowsShort>;
+        auto by_rows = rows == kRowsWhole    ? f8_quantize_tile_kernel<TYPE, false, kRowsWhole>
+                       : rows == kRowsRagged ? f8_quantize_tile_kernel<TYPE, false, kRowsRagged>
+                                             : f8_quantize_tile_kernel<TYPE, false, kRowsShort>;
+        auto kern = block_rows == 1 ? by_rows : square;
         hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), 0, g_rt.stream, x, (size_t)ldx, M, K, e5m2, e8m0, Q, (size_t)ldq, S,
                            (size_t)lds, Qt, (size_t)ldqt, St, (size_t)ldst, col_blocks);
     }

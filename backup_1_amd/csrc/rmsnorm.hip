@@ -46,7 +46,7 @@ struct RmsNormArgs {
     int M, K, e5m2, e8m0;
 };
 
-template <int TYPE, int NT, int CH, bool WHOLE>
+template <int TYPE, int NT, int CH, int ROWS>
 __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
     typedef typename Wide<TYPE>::T T;
     __shared__ float part[NT / kWave];
@@ -57,16 +57,16 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-        raw_x[i] = fetch8_part<TYPE, false, WHOLE>(x + at, K - k, k);
-        if (g.R) raw_r[i] = fetch8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k, k);
+        raw_x[i] = fetch8_part<TYPE, ROWS>(x + at, K - k);
+        if (g.R) raw_r[i] = fetch8_part<TYPE, ROWS>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k);
     }
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int k = 8 * ((int)threadIdx.x + i * NT);
-        settle8_part<TYPE, WHOLE>(raw_x[i], K - k, k);
+        settle8_part<TYPE, ROWS>(raw_x[i], K - k);
         h[i] = widen8<TYPE>(raw_x[i]);
         if (g.R) {
-            settle8_part<TYPE, WHOLE>(raw_r[i], K - k, k);
+            settle8_part<TYPE, ROWS>(raw_r[i], K - k);
             const Eight r = widen8<TYPE>(raw_r[i]);
             // the sum is what the stream carries on, so it is rounded to its type here and the norm is taken of that
 #pragma unroll
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-        const Eight w = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.W) + at, K - k, k);
+        const Eight w = load8_part<TYPE, ROWS>(static_cast<const T*>(g.W) + at, K - k);
         Eight y;
 #pragma unroll
         for (int e = 0; e < 8; ++e) y.v[e] = h[i].v[e] * rstd * w.v[e];     // in this order: |h * rstd| <= sqrt(K), h * w may overflow
@@ -128,7 +128,7 @@ struct RmsNormBackwardArgs {
 // there is one launch and no workspace.  For few rows of inputs that the caches hold (rmsnorm_backward_enqueue).  64 rows a
 // pass and four passes in flight; columns for that many lanes.
 constexpr int dw_columns(int nt) { return nt / 8 < 64 ? nt / 8 : 64; }
-template <int TYPE, int NT, bool WHOLE>
+template <int TYPE, int NT, int ROWS>
 __device__ __forceinline__ void rmsnorm_dw_columns(const RmsNormBackwardArgs& g, int group) {
     typedef typename Wide<TYPE>::T T;
     constexpr int COLS = dw_columns(NT), LANES = COLS / 8, GROUPS = NT / LANES, AHEAD = 4;
@@ -142,13 +142,13 @@ __device__ __forceinline__ void rmsnorm_dw_columns(const RmsNormBackwardArgs& g,
         for (int j = 0; j < AHEAD; ++j) {
             const int m = m0 + GROUPS * j, row = m < g.M ? m : 0;
             rstd[j] = m < g.M ? g.rstd[row] : 0.f;
-            h[j] = fetch8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.H) + (size_t)row * g.ldh + at, m < g.M ? g.K - k : 0, k);
-            dy[j] = fetch8_part<TYPE, false, WHOLE>(static_cast<const T*>(g.dY) + (size_t)row * g.lddy + at, m < g.M ? g.K - k : 0, k);
+            h[j] = fetch8_part<TYPE, ROWS>(static_cast<const T*>(g.H) + (size_t)row * g.ldh + at, m < g.M ? g.K - k : 0);
+            dy[j] = fetch8_part<TYPE, ROWS>(static_cast<const T*>(g.dY) + (size_t)row * g.lddy + at, m < g.M ? g.K - k : 0);
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            settle8_part<TYPE, WHOLE>(h[j], g.K - k, k);            // rows past the last are zeros either way
-            settle8_part<TYPE, WHOLE>(dy[j], g.K - k, k);
+            settle8_part<TYPE, ROWS>(h[j], g.K - k);            // rows past the last are zeros either way
+            settle8_part<TYPE, ROWS>(dy[j], g.K - k);
             const Eight hv = widen8<TYPE>(h[j]), yv = widen8<TYPE>(dy[j]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] = __builtin_fmaf(yv.v[e], hv.v[e] * rstd[j], sum[e]);
@@ -173,12 +173,12 @@ __device__ __forceinline__ void rmsnorm_dw_columns(const RmsNormBackwardArgs& g,
 
 // Workgroup b owns rows b * rows_each ...: their dx, and their part of dw in a row of `partial`, which the second kernel
 // adds up in row order (no atomics: the same bits on every run).
-template <int TYPE, int NT, int CH, bool WHOLE>
+template <int TYPE, int NT, int CH, int ROWS>
 __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward_kernel(const RmsNormBackwardArgs g) {
     typedef typename Wide<TYPE>::T T;
     __shared__ float part[2][NT / kWave];
     if ((int)blockIdx.x >= g.row_groups) {
-        rmsnorm_dw_columns<TYPE, NT, WHOLE>(g, (int)blockIdx.x - g.row_groups);
+        rmsnorm_dw_columns<TYPE, NT, ROWS>(g, (int)blockIdx.x - g.row_groups);
         return;
     }
     const int K = g.K, first = (int)blockIdx.x * g.rows_each;
@@ -199,9 +199,9 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            r.h[i] = fetch8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k, k);
-            r.dy[i] = fetch8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k, k);
-            if (g.dR) r.dr[i] = fetch8_part<TYPE, STREAM, WHOLE>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k, k);
+            r.h[i] = fetch8_part<TYPE, ROWS, STREAM>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k);
+            r.dy[i] = fetch8_part<TYPE, ROWS, STREAM>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k);
+            if (g.dR) r.dr[i] = fetch8_part<TYPE, ROWS, STREAM>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
         }
     };
     auto load_row = [&](Row& r, int m) {
@@ -219,9 +219,9 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            const Eight w = load8_part<TYPE, WHOLE>(static_cast<const T*>(g.W) + at, K - k, k);
-            settle8_part<TYPE, WHOLE>(row.h[i], K - k, k);
-            settle8_part<TYPE, WHOLE>(row.dy[i], K - k, k);
+            const Eight w = load8_part<TYPE, ROWS>(static_cast<const T*>(g.W) + at, K - k);
+            settle8_part<TYPE, ROWS>(row.h[i], K - k);
+            settle8_part<TYPE, ROWS>(row.dy[i], K - k);
             n[i] = widen8<TYPE>(row.h[i]);
             dn[i] = widen8<TYPE>(row.dy[i]);
 #pragma unroll
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
 #pragma unroll
             for (int e = 0; e < 8; ++e) dx.v[e] = rstd * __builtin_fmaf(-n[i].v[e], mean, dn[i].v[e]);
             if (g.dR) {
-                settle8_part<TYPE, WHOLE>(row.dr[i], K - k, k);
+                settle8_part<TYPE, ROWS>(row.dr[i], K - k);
                 const Eight dr = widen8<TYPE>(row.dr[i]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dx.v[e] += dr.v[e];
@@ -325,23 +325,28 @@ static int rmsnorm_f8_launch(const RmsNormArgs& g) {
     // a workgroup a row
     if ((long)g.M * (g.K <= 512 ? 64 : g.K <= 1024 ? 128 : g.K <= 8192 ? 256 : g.K <= 16384 ? 512 : 1024) > kMostThreads)
         return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
-    const bool whole = g.K % 8 == 0;
-#define DECX_LAUNCH(NT, CH) \
-    hipLaunchKernelGGL((whole ? rmsnorm_f8_kernel<TYPE, NT, CH, true> : rmsnorm_f8_kernel<TYPE, NT, CH, false>), dim3((unsigned)g.M), dim3(NT), 0, g_rt.stream, g)
-    DECX_RMSNORM_SHAPES(g.K, 4, DECX_LAUNCH);
+    const int rows = rows_kind(g.K);
+#define DECX_LAUNCH(NT, CH)                                                                                                          \
+    hipLaunchKernelGGL((rows == kRowsWhole ? rmsnorm_f8_kernel<TYPE, NT, CH, kRowsWhole> : rmsnorm_f8_kernel<TYPE, NT, CH, kRowsRagged>), \
+                       dim3((unsigned)g.M), dim3(NT), 0, g_rt.stream, g)
+    if (rows == kRowsShort) hipLaunchKernelGGL((rmsnorm_f8_kernel<TYPE, kWave, 1, kRowsShort>), dim3((unsigned)g.M), dim3(kWave), 0, g_rt.stream, g);
+    else DECX_RMSNORM_SHAPES(g.K, 4, DECX_LAUNCH);
 #undef DECX_LAUNCH
     HIP_TRY(hipGetLastError());
     return 0;
 }
 template <int TYPE>
 static int rmsnorm_backward_launch(const RmsNormBackwardArgs& g) {
-    const bool whole = g.K % 8 == 0;        // rows of whole chunks: no other way of loading beside theirs, which costs registers
-#define DECX_LAUNCH(NT, CH)                                                                                                    \
-    hipLaunchKernelGGL((whole ? rmsnorm_backward_kernel<TYPE, NT, CH, true> : rmsnorm_backward_kernel<TYPE, NT, CH, false>),       \
-                       dim3((unsigned)(g.row_groups + (g.dW ? cdiv(g.K, dw_columns(NT)) : 0))), dim3(NT), 0, g_rt.stream, g)
+    const int rows = rows_kind(g.K);
+#define DECX_GRID(NT) dim3((unsigned)(g.row_groups + (g.dW ? cdiv(g.K, dw_columns(NT)) : 0)))
+#define DECX_LAUNCH(NT, CH)                                                                                                                  \
+    hipLaunchKernelGGL((rows == kRowsWhole ? rmsnorm_backward_kernel<TYPE, NT, CH, kRowsWhole> : rmsnorm_backward_kernel<TYPE, NT, CH, kRowsRagged>), \
+                       DECX_GRID(NT), dim3(NT), 0, g_rt.stream, g)
     constexpr int MOST = TYPE == 0 ? 2 : 4;
-    DECX_RMSNORM_SHAPES(g.K, MOST, DECX_LAUNCH);
+    if (rows == kRowsShort) hipLaunchKernelGGL((rmsnorm_backward_kernel<TYPE, kWave, 1, kRowsShort>), DECX_GRID(kWave), dim3(kWave), 0, g_rt.stream, g);
+    else DECX_RMSNORM_SHAPES(g.K, MOST, DECX_LAUNCH);
 #undef DECX_LAUNCH
+#undef DECX_GRID
     HIP_TRY(hipGetLastError());
     return 0;
 }
