@@ -177,20 +177,36 @@ template <int TYPE, int NT, int CH, int ROWS>
 __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward_kernel(const RmsNormBackwardArgs g) {
     typedef typename Wide<TYPE>::T T;
     __shared__ float part[2][NT / kWave];
-    if ((int)blockIdx.x >= g.row_groups) {
-        rmsnorm_dw_columns<TYPE, NT, ROWS>(g, (int)blockIdx.x - g.row_groups);
-        return;
+    // The thread's columns of dw: in registers, or, where a thread has 128 of them and 4 chunks, in LDS, in whole vectors of the
+    // workgroup one after the other
+    constexpr bool DW_IN_LDS = NT >= 1024 && CH == 4;
+    if constexpr (!DW_IN_LDS) {                                 // (LDS has no room for the columns' sums beside that)
+        if ((int)blockIdx.x >= g.row_groups) {
+            rmsnorm_dw_columns<TYPE, NT, ROWS>(g, (int)blockIdx.x - g.row_groups);
+            return;
+        }
     }
     const int K = g.K, first = (int)blockIdx.x * g.rows_each;
     const int last = first + g.rows_each < g.M ? first + g.rows_each : g.M;
-    Eight dw[CH];
+    __shared__ f32x4 dw_lds[DW_IN_LDS ? 2 * CH * NT : 1];
+    Eight dw[DW_IN_LDS ? 1 : CH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
+    for (int i = 0; i < CH; ++i) {
+        if (DW_IN_LDS) {
+            dw_lds[2 * i * NT + threadIdx.x] = f32x4{0.f, 0.f, 0.f, 0.f};
+            dw_lds[(2 * i + 1) * NT + threadIdx.x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dw[i].v[e] = 0.f;
-    // the next row's loads are in flight while a row waits for its sum
+            for (int e = 0; e < 8; ++e) dw[i].v[e] = 0.f;
+        }
+    }
+    // The next row's loads are in flight while a row waits for its sum.  Not where a workgroup fills the CU and a thread has 128
+    // registers (LONG): there a row stays as it was loaded, n and g are made twice, and dr is fetched when it is added.  With all
+    // of that in registers, and so in scratch memory, 2048 x 32768 bf16 took 448 us; so, and with dw in LDS, 119.  n and g are
+    // also made twice (TWICE) where the moving of row ends would cost the last registers (2048 x 12001 bf16 62.3 -> 58.5 us).
+    constexpr bool LONG = NT >= 1024, TWICE = LONG || (TYPE != 0 && CH == 4 && ROWS == kRowsRagged);
     struct Row {
-        RawEight<TYPE> h[CH], dy[CH], dr[CH];
+        RawEight<TYPE> h[CH], dy[CH], dr[LONG ? 1 : CH];
         float rstd;
     };
     auto load_row_as = [&](Row& r, int m, auto stream_tag) {
@@ -201,7 +217,7 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
             r.h[i] = fetch8_part<TYPE, ROWS, STREAM>(static_cast<const T*>(g.H) + (size_t)m * g.ldh + at, K - k);
             r.dy[i] = fetch8_part<TYPE, ROWS, STREAM>(static_cast<const T*>(g.dY) + (size_t)m * g.lddy + at, K - k);
-            if (g.dR) r.dr[i] = fetch8_part<TYPE, ROWS, STREAM>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
+            if (g.dR && !LONG) r.dr[i] = fetch8_part<TYPE, ROWS, STREAM>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
         }
     };
     auto load_row = [&](Row& r, int m) {
@@ -209,40 +225,63 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
         else load_row_as(r, m, std::false_type{});
     };
     Row next;
-    load_row(next, first);
+    if (!LONG) load_row(next, first);
     for (int m = first; m < last; ++m) {
+        if (LONG) load_row(next, m);
         Row row = next;
-        if (m + 1 < last) load_row(next, m + 1);
+        if (!LONG && m + 1 < last) load_row(next, m + 1);
         const float rstd = row.rstd;
-        Eight n[CH], dn[CH];                                    // n and g
+        Eight n[TWICE ? 1 : CH], dn[TWICE ? 1 : CH];            // n and g; TWICE: of a chunk at a time
+        auto weigh = [&](int i, Eight& ni, Eight& gi, bool first_time) {
+            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+            const Eight w = load8_part<TYPE, ROWS>(static_cast<const T*>(g.W) + at, K - k);
+            ni = widen8<TYPE>(row.h[i]);
+            gi = widen8<TYPE>(row.dy[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ni.v[e] *= rstd;
+            if (first_time && DW_IN_LDS) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    f32x4 sums = dw_lds[(2 * i + half) * NT + threadIdx.x];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sums[e] = __builtin_fmaf(gi.v[4 * half + e], ni.v[4 * half + e], sums[e]);
+                    dw_lds[(2 * i + half) * NT + threadIdx.x] = sums;
+                }
+            } else if (first_time) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dw[i].v[e] = __builtin_fmaf(gi.v[e], ni.v[e], dw[i].v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gi.v[e] *= w.v[e];
+        };
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-            const Eight w = load8_part<TYPE, ROWS>(static_cast<const T*>(g.W) + at, K - k);
+            const int k = 8 * ((int)threadIdx.x + i * NT);
             settle8_part<TYPE, ROWS>(row.h[i], K - k);
             settle8_part<TYPE, ROWS>(row.dy[i], K - k);
-            n[i] = widen8<TYPE>(row.h[i]);
-            dn[i] = widen8<TYPE>(row.dy[i]);
+            Eight &ni = n[TWICE ? 0 : i], &gi = dn[TWICE ? 0 : i];
+            weigh(i, ni, gi, true);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                n[i].v[e] *= rstd;
-                dw[i].v[e] = __builtin_fmaf(dn[i].v[e], n[i].v[e], dw[i].v[e]);
-                dn[i].v[e] *= w.v[e];
-                sum = __builtin_fmaf(dn[i].v[e], n[i].v[e], sum);
-            }
+            for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(gi.v[e], ni.v[e], sum);
         }
         // two sets of partial sums in turn: a wave may be a row ahead of another, never two (it meets it in between)
         const float mean = __fdiv_rn(workgroup_sum<NT>(sum, part[m & 1]), (float)K);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+            Eight &ni = n[TWICE ? 0 : i], &gi = dn[TWICE ? 0 : i];
+            if (TWICE) {
+                if (LONG && g.dR) row.dr[0] = fetch8_part<TYPE, ROWS>(static_cast<const T*>(g.dR) + (size_t)m * g.lddr + at, K - k);
+                weigh(i, ni, gi, false);
+            }
             Eight dx;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dx.v[e] = rstd * __builtin_fmaf(-n[i].v[e], mean, dn[i].v[e]);
+            for (int e = 0; e < 8; ++e) dx.v[e] = rstd * __builtin_fmaf(-ni.v[e], mean, gi.v[e]);
             if (g.dR) {
-                settle8_part<TYPE, ROWS>(row.dr[i], K - k);
-                const Eight dr = widen8<TYPE>(row.dr[i]);
+                RawEight<TYPE>& raw = row.dr[LONG ? 0 : i];
+                settle8_part<TYPE, ROWS>(raw, K - k);
+                const Eight dr = widen8<TYPE>(raw);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dx.v[e] += dr.v[e];
             }
@@ -253,7 +292,12 @@ __global__ __launch_bounds__(NT, NT >= 512 ? NT / 256 : 2) void rmsnorm_backward
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int k = 8 * ((int)threadIdx.x + i * NT);
-        store8_part<0>(g.partial + (size_t)blockIdx.x * K + (k < K ? k : 0), dw[i], K - k);
+        Eight sums = dw[DW_IN_LDS ? 0 : i];
+        if (DW_IN_LDS) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sums.v[e] = dw_lds[(2 * i + e / 4) * NT + threadIdx.x][e % 4];
+        }
+        store8_part<0>(g.partial + (size_t)blockIdx.x * K + (k < K ? k : 0), sums, K - k);
     }
 }
 
@@ -378,13 +422,15 @@ int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const voi
     return rmsnorm_f8_launch<2>(g);
 }
 
-// Workgroups of the gradient: as many as keep about 32 KB of each input on a compute unit, 2 to 8 a unit (short rows wait for
-// memory one after the other: 8192 x 256 took 24 us with 2, 17.5 with 8; long fp32 ones gain nothing: 8192 x 4096 114 us
-// with 2, 123 with 4), and none without rows.  The workspace is sized for the 2-byte types.
+// Workgroups of the gradient.  More of them hide more of the wait for a row's sum, but each writes a row of `partial`, so there
+// are fewer the longer the rows are, and not many for few rows: 4 rows each from 512 workgroups on.  2048 x 2048 bf16 takes
+// 22.4 us with a row each and 13.5 with 4; of 8192 rows, 256 elements 14 us with 2048 workgroups and 18 with 512, 2048
+// elements 36 and 29; 2048 x 8192 fp32 62 us with 256 and 66 with 512.  The workspace is sized for the 2-byte types.
 static int rmsnorm_backward_groups(int M, int K, int size) {
-    const int held = K <= 512 ? 512 : K <= 1024 ? 1024 : K <= 2048 ? 2048 : K <= 4096 ? 4096 : 8192;
-    const int fit = 32768 / (held * size), each = fit < 2 ? 2 : fit > 8 ? 8 : fit;
-    const int most = each * (g_rt.compute_units > 0 ? g_rt.compute_units : 256);
+    const long bytes = (long)K * size;
+    const int each = bytes <= 1024 ? 8 : bytes <= 2048 ? 4 : bytes <= 4096 ? 3 : bytes <= 16384 ? 2 : 1;
+    const int cus = g_rt.compute_units > 0 ? g_rt.compute_units : 256;
+    const int by_rows = cdiv(M, 4) > 2 * cus ? cdiv(M, 4) : 2 * cus, most = each * cus < by_rows ? each * cus : by_rows;
     const int groups = M < most ? M : most;
     return cdiv(M, cdiv(M, groups));
 }
@@ -414,7 +460,7 @@ int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float*
     // Few rows of inputs that the caches hold: the column workgroups (one launch: 200 x 1500 8.4 -> 5.6 us, 512 x 4096 10.7 ->
     // 7.4, 512 x 8192 15.9 -> 13; 2048 x 512 would go 12.5 -> 29.8), unless dX overwrites what they read
     const bool in_place = dX == H || dX == dY;
-    const bool columns = dW && !in_place && M <= 512 && (size_t)M * K <= (size_t)1 << 22;
+    const bool columns = dW && !in_place && M <= 512 && (size_t)M * K <= (size_t)1 << 22 && K <= kRmsNormMaxK / 2;      // DW_IN_LDS beyond
     if (columns) g.dW = dW;
     else if (dW) g.partial = static_cast<float*>(work);
     g.ldh = (size_t)ldh, g.lddy = (size_t)lddy, g.lddr = (size_t)lddr, g.lddx = (size_t)lddx;

@@ -156,3 +156,12 @@ def test_refusals(gpu):
     refused(0x0d, X=d.ptr + 2)
     refused(0x0d, X=d.ptr + 1, type=capi.F16)
     refused(0x0d, S=d.ptr + 32769)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+@pytest.mark.parametrize("K", range(1, 18))
+def test_each_short_row(gpu, kind, K):
+    x = values(9, K, kind, 60 + K)
+    for block_rows in (1, 128):
+        check(x, kind, capi.E4M3, capi.SCALE_F32, block_rows, run(x, kind, capi.E4M3, capi.SCALE_F32, block_rows, True, True, (3, 1, 0), (1, 1, 0)))
+    check(x, kind, capi.E5M2, capi.SCALE_E8M0, 1, run(x, kind, capi.E5M2, capi.SCALE_E8M0, 1, False))

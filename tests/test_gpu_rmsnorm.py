@@ -277,3 +277,27 @@ def test_integers_beyond_an_int_are_refused(gpu, call):
         else:
             capi.rmsnorm_backward(d.ptr, 16, d.ptr, d.ptr, d.ptr, 16, None, 0, 0, 1, 1, d.ptr, far + 16, None, None, 0)
     assert e.value.code == 0x0d and "no int" in str(e.value)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+@pytest.mark.parametrize("M,K", [(3, 9001), (5, 20001), (300, 16400), (1030, 40)])
+def test_gradient_of_long_rows_in_place(gpu, kind, M, K):
+    """Rows that a workgroup of 1024 holds: results over each input, the sums of several rows a workgroup; the same bits as apart."""
+    h, dy, w = inputs(M, K, kind, 21)
+    dr = ref.to_type(workloads.normal((M, K), 79), kind)
+    rstd = (1 / np.sqrt((ref.from_type(h, kind) ** 2).mean(1) + EPS)).astype(np.float32)
+    plain = backward(h, w, rstd, dy, dr, kind)
+    check_backward(h, w, rstd, dy, dr, kind, plain, M)
+    for where in ("h", "y", "r"):
+        got = backward(h, w, rstd, dy, dr, kind, inplace=where, pitch=5)
+        assert np.array_equal(got[0].view(np.uint8), plain[0].view(np.uint8))
+        check_backward(h, w, rstd, dy, dr, kind, got, M)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+@pytest.mark.parametrize("K", range(1, 18))
+def test_each_short_row(gpu, kind, K):
+    x, r, w = inputs(5, K, kind, 200 + K)
+    check(x, r, w, kind, run(x, r, w, kind, pitch=3, lead=1))
+    rstd = (1 / np.sqrt((ref.from_type(x, kind) ** 2).mean(1) + EPS)).astype(np.float32)
+    check_backward(x, w, rstd, r, None, kind, backward(x, w, rstd, r, None, kind, pitch=1, lead=1), 5)
