@@ -43,7 +43,7 @@ struct RmsNormArgs {
     void* S;
     size_t ldx, ldr, ldh, ldy, ldq, lds;
     float eps;
-    int M, K, e5m2, e8m0;
+    int M, K, e5m2, e8m0, stream;
 };
 
 template <int TYPE, int NT, int CH, int ROWS>
@@ -54,12 +54,17 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
     const T* x = static_cast<const T*>(g.X) + (size_t)m * g.ldx;
     Eight h[CH];
     RawEight<TYPE> raw_x[CH], raw_r[CH];
+    auto load_row = [&](auto stream_tag) {
+        constexpr bool STREAM = decltype(stream_tag)::value;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
-        raw_x[i] = fetch8_part<TYPE, ROWS>(x + at, K - k);
-        if (g.R) raw_r[i] = fetch8_part<TYPE, ROWS>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k);
-    }
+        for (int i = 0; i < CH; ++i) {
+            const int k = 8 * ((int)threadIdx.x + i * NT), at = k < K ? k : 0;
+            raw_x[i] = fetch8_part<TYPE, ROWS, STREAM>(x + at, K - k);
+            if (g.R) raw_r[i] = fetch8_part<TYPE, ROWS, STREAM>(static_cast<const T*>(g.R) + (size_t)m * g.ldr + at, K - k);
+        }
+    };
+    if (TYPE != 0 && g.stream) load_row(std::true_type{});
+    else load_row(std::false_type{});
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int k = 8 * ((int)threadIdx.x + i * NT);
@@ -121,7 +126,7 @@ struct RmsNormBackwardArgs {
     int row_groups;           // workgroups of rows; those behind them take columns of dW
     size_t ldh, lddy, lddr, lddx;
     int M, K, rows_each;
-    int stream;               // the inputs are larger than the memory-side cache
+    int stream;               // the inputs are more than the caches keep
 };
 
 // dw of some columns straight from H and dY, in workgroups of their own beside those of the rows: both are read twice, but
@@ -416,6 +421,9 @@ int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const voi
     RmsNormArgs g = {};
     g.X = X, g.R = R, g.W = W, g.H = H, g.Y = Y, g.rstd = rstd, g.Q = Q, g.S = S;
     g.ldx = (size_t)ldx, g.ldr = (size_t)ldr, g.ldh = (size_t)ldh, g.ldy = (size_t)ldy, g.ldq = (size_t)ldq, g.lds = (size_t)lds;
+    // 16-bit inputs of more than 96 MiB are read past the caches, which hold them no longer with the results: 8192 x 8192, 268 MB,
+    // 121 us against 133, 8192 x 4096 54 against 61; 4096 x 4096, 67 MB, 29 against 24
+    g.stream = (size_t)M * K * (R ? 4 : 2) > ((size_t)96 << 20);
     g.eps = eps, g.M = M, g.K = K, g.e5m2 = format == DECX_HIP_E5M2, g.e8m0 = scale_type == DECX_HIP_SCALE_E8M0;
     if (type == DECX_HIP_F32) return rmsnorm_f8_launch<0>(g);
     if (type == DECX_HIP_F16) return rmsnorm_f8_launch<1>(g);
@@ -465,9 +473,9 @@ int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float*
     else if (dW) g.partial = static_cast<float*>(work);
     g.ldh = (size_t)ldh, g.lddy = (size_t)lddy, g.lddr = (size_t)lddr, g.lddx = (size_t)lddx;
     g.M = M, g.K = K, g.rows_each = cdiv(M, groups);
-    // 16-bit inputs of more than the memory-side cache's 256 MiB are read past the caches: 8192 x 8192, 402 MB, 104 us
-    // against 112; 8192 x 1000, 49 MB, 36 against 31 (and in fp32, whose lanes read a line in two pieces, always slower)
-    g.stream = (size_t)M * K * (dR ? 6 : 4) > ((size_t)256 << 20);
+    // 16-bit inputs of more than 128 MiB are read past the caches: 8192 x 8192, 402 MB, 99 us against 112, 4096 x 8192, 201 MB, 55
+    // against 61; 2048 x 8192, 101 MB, 32 against 29 (and in fp32, whose lanes read a line in two pieces, always slower)
+    g.stream = (size_t)M * K * (dR ? 6 : 4) > ((size_t)128 << 20);
     int rc = type == DECX_HIP_F32 ? rmsnorm_backward_launch<0>(g) : type == DECX_HIP_F16 ? rmsnorm_backward_launch<1>(g) : rmsnorm_backward_launch<2>(g);
     if (rc || !g.partial) return rc;
     if (K <= 2048)          // narrow pieces where wide ones would leave most of the chip idle
