@@ -375,9 +375,14 @@ static int rmsnorm_f8_launch(const RmsNormArgs& g) {
     if ((long)g.M * (g.K <= 512 ? 64 : g.K <= 1024 ? 128 : g.K <= 8192 ? 256 : g.K <= 16384 ? 512 : 1024) > kMostThreads)
         return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
     const int rows = rows_kind(g.K);
+    // Long rows (8 to 32 KB) from memory: 4 workgroups a CU instead of 8, by LDS that nothing uses.  8 have twice the loads in
+    // flight that memory needs, from twice the places: 8192 x 8192 bf16 132 us against 119, 4096 x 8192 fp32 134 against 126.
+    // Where the caches hold the inputs, 8 are better (1262 x 8192 bf16 16.5 against 17.7), and with shorter rows.
+    const size_t row_bytes = (size_t)g.K * sizeof(typename Wide<TYPE>::T), inputs = (size_t)g.M * row_bytes * (g.R ? 2 : 1);
+    const size_t unused = row_bytes > 8192 && g.K <= 8192 && inputs >= (size_t)64 << 20 ? 40000 : 0;
 #define DECX_LAUNCH(NT, CH)                                                                                                          \
     hipLaunchKernelGGL((rows == kRowsWhole ? rmsnorm_f8_kernel<TYPE, NT, CH, kRowsWhole> : rmsnorm_f8_kernel<TYPE, NT, CH, kRowsRagged>), \
-                       dim3((unsigned)g.M), dim3(NT), 0, g_rt.stream, g)
+                       dim3((unsigned)g.M), dim3(NT), unused, g_rt.stream, g)
     if (rows == kRowsShort) hipLaunchKernelGGL((rmsnorm_f8_kernel<TYPE, kWave, 1, kRowsShort>), dim3((unsigned)g.M), dim3(kWave), 0, g_rt.stream, g);
     else DECX_RMSNORM_SHAPES(g.K, 4, DECX_LAUNCH);
 #undef DECX_LAUNCH
@@ -421,9 +426,11 @@ int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const voi
     RmsNormArgs g = {};
     g.X = X, g.R = R, g.W = W, g.H = H, g.Y = Y, g.rstd = rstd, g.Q = Q, g.S = S;
     g.ldx = (size_t)ldx, g.ldr = (size_t)ldr, g.ldh = (size_t)ldh, g.ldy = (size_t)ldy, g.ldq = (size_t)ldq, g.lds = (size_t)lds;
-    // 16-bit inputs of more than 96 MiB are read past the caches, which hold them no longer with the results: 8192 x 8192, 268 MB,
-    // 121 us against 133, 8192 x 4096 54 against 61; 4096 x 4096, 67 MB, 29 against 24
-    g.stream = (size_t)M * K * (R ? 4 : 2) > ((size_t)96 << 20);
+    // 16-bit inputs of 96 to 256 MiB are read past the caches, whose 256 MiB the results then have for themselves: 4096 x 8192,
+    // 134 MB, 64 us against 68 (59 against 65 where little else is used in between); 4096 x 4096, 67 MB, 29 against 24, and
+    // 8192 x 8192, 268 MB, 125 against 119
+    const size_t inputs = (size_t)M * K * (R ? 4 : 2);
+    g.stream = inputs > ((size_t)96 << 20) && inputs < ((size_t)256 << 20);
     g.eps = eps, g.M = M, g.K = K, g.e5m2 = format == DECX_HIP_E5M2, g.e8m0 = scale_type == DECX_HIP_SCALE_E8M0;
     if (type == DECX_HIP_F32) return rmsnorm_f8_launch<0>(g);
     if (type == DECX_HIP_F16) return rmsnorm_f8_launch<1>(g);
