@@ -31,7 +31,7 @@ struct RawEight {
     u32x4 w[TYPE == 0 ? 2 : 1];
 };
 // STREAM: non-temporal, for inputs that no cache can hold.  Stores of 16-bit types are non-temporal always (norm of 8192 x
-// 8192 134 -> 127 us); those of fp32, a lane's 32 bytes in two, leave half lines that way (8192 x 4096 100 -> 119).
+// 8192: 5 % faster); those of fp32, a lane's 32 bytes in two, leave half lines that way (8192 x 4096 100 -> 119).
 template <int TYPE, bool STREAM = false>
 __device__ __forceinline__ RawEight<TYPE> load_raw8(const typename Wide<TYPE>::T* p) {
     RawEight<TYPE> r;
