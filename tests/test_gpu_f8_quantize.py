@@ -165,3 +165,16 @@ def test_each_short_row(gpu, kind, K):
     for block_rows in (1, 128):
         check(x, kind, capi.E4M3, capi.SCALE_F32, block_rows, run(x, kind, capi.E4M3, capi.SCALE_F32, block_rows, True, True, (3, 1, 0), (1, 1, 0)))
     check(x, kind, capi.E5M2, capi.SCALE_E8M0, 1, run(x, kind, capi.E5M2, capi.SCALE_E8M0, 1, False))
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_matrix_larger_than_the_caches(gpu, block_rows):
+    """104 MB of fp32, where fewer workgroups share a unit: 5 copies of 1024 rows give 5 copies of their codes and scales."""
+    M, K, times = 1024, 5080, 5
+    x = values(M, K, capi.F32, 95)
+    got = run(np.tile(x, (times, 1)), capi.F32, capi.E4M3, capi.SCALE_F32, block_rows)
+    rows = got[1].shape[1] // times
+    want = ref.quantize(x, capi.E4M3, capi.SCALE_F32, block_rows)
+    assert np.array_equal(got[0], np.tile(want[0], (times, 1))) and np.array_equal(got[1], np.tile(want[1], (1, times))) and rows == want[1].shape[1]
+    want = ref.quantize(x.T.copy(), capi.E4M3, capi.SCALE_F32, block_rows)
+    assert np.array_equal(got[2], np.tile(want[0], (1, times))) and np.array_equal(got[3], np.tile(want[1], (times, 1)))

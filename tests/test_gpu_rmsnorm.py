@@ -301,3 +301,23 @@ def test_each_short_row(gpu, kind, K):
     check(x, r, w, kind, run(x, r, w, kind, pitch=3, lead=1))
     rstd = (1 / np.sqrt((ref.from_type(x, kind) ** 2).mean(1) + EPS)).astype(np.float32)
     check_backward(x, w, rstd, r, None, kind, backward(x, w, rstd, r, None, kind, pitch=1, lead=1), 5)
+
+
+@pytest.mark.parametrize("kind,M,K,times", [(capi.BF16, 700, 8192, 6), (capi.F16, 900, 8192, 10), (capi.F32, 500, 8190, 9)])
+def test_inputs_larger_than_the_caches(gpu, kind, M, K, times):
+    """More than 96 MiB, where loads and workgroups a unit are chosen otherwise: some rows against 64 bits, the same rows again and
+    again in the same bits."""
+    x, r, w = inputs(M, K, kind, 90)
+    big = lambda a: np.tile(a, (times, 1))  # noqa: E731
+    got = run(big(x), big(r), w, kind)
+    first = {n: (v[:, :M] if n in ("rstd", "S") else v[:M]) for n, v in got.items()}
+    check(x, r, w, kind, first)
+    for n, v in got.items():
+        want = np.tile(first[n], (1, times)) if n in ("rstd", "S") else big(first[n])
+        assert np.array_equal(v.view(np.uint8), want.view(np.uint8)), n
+    rstd = first["rstd"][0]
+    dx, dw = backward(big(x), w, np.tile(rstd, times), big(r), big(r), kind)
+    check_backward(x, w, rstd, r, r, kind, (dx[:M], None), M)
+    assert np.array_equal(dx.view(np.uint8), big(dx[:M]).view(np.uint8))
+    _, _, want_w, size_w = gradient64(ref.from_type(x, kind), ref.from_type(w, kind), rstd.astype(np.float64), ref.from_type(r, kind), 0.0)
+    assert np.all(np.abs(dw - times * want_w) <= times * size_w * (times * M + 20) * 2.0 ** -24)
