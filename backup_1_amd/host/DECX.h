@@ -234,7 +234,8 @@ DH GEMM3(MatrixArray<Half>& A, MatrixArray<Half>& B, MatrixArray<Half>& C, Matri
 // size and scales (M / block_rows wide, K / 128 high, both rounded up; block_rows 1 or 128), fp32 or -- in a uchar matrix --
 // biased exponents of powers of two; Quantize_f8_T does the same of the transpose.  GEMM_f8 multiplies A (K wide, M high,
 // scaled by rows) with B, which holds one column of the product per row (K wide, N high) and is scaled by rows or by 128
-// rows, whichever its scales' width says: dst (N wide, M high) = A * B^T.
+// rows, whichever its scales' width says: dst (N wide, M high) = A * B^T.  A result may be a container that the call reads, or
+// share its block: it then gets a block of its own.  One container cannot be two results.
 DH Quantize_f8(GPU_Matrix<float>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int block_rows, const int format);
 DH Quantize_f8(GPU_Matrix<Half>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int block_rows, const int format);
 DH Quantize_f8(GPU_Matrix<float>& src, GPU_Matrix<uchar>& codes, GPU_Matrix<uchar>& scales, const int block_rows, const int format);

@@ -7,6 +7,7 @@
 // rejects unknown flags (the reference returns an unfilled DH, conv2_mk_im2col.h:301-305).
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "decx_classes.hpp"
 
@@ -475,6 +476,30 @@ DH size_output(decx::_GPU_Matrix<T>* m, uint w, uint h) {
     return m->last_status == DECX_HIP_FAIL_ALLOCATION ? alloc_fail() : from_status(m->last_status);
 }
 
+// A result of a call: the caller's container, or, where that is one that the call reads (or another of its results) or shares
+// its block with such a one, a fresh container that it then takes over, as gemm_device's dst.  Sized in place it would free or
+// resize what the kernel reads.  Containers of one block always have one size, so a result may stay in place over an input
+// that its kernel reads element by element before it writes.
+template <typename T>
+class F8Output {
+    decx::_GPU_Matrix<T>* to_;
+    decx::_GPU_Matrix<T> fresh_;
+    bool apart_ = false;
+
+public:
+    explicit F8Output(decx::_GPU_Matrix<T>* to) : to_(to) {}
+    template <typename U>
+    F8Output& keep_off(const decx::_GPU_Matrix<U>* other) {
+        if constexpr (std::is_same_v<T, U>) apart_ = apart_ || to_ == other || to_->shares_block_with(*other);
+        return *this;
+    }
+    DH size(uint w, uint h) { return size_output(apart_ ? &fresh_ : to_, w, h); }
+    decx::_GPU_Matrix<T>* operator->() { return apart_ ? &fresh_ : to_; }
+    void take_over() {
+        if (apart_) to_->share_from(fresh_);
+    }
+};
+
 template <typename T, typename S>
 DH quantize_f8(GPU_Matrix<T>& src_, GPU_Matrix<uchar>& codes_, GPU_Matrix<S>& scales_, int block_rows, int format, bool transpose) {
     auto* src = dynamic_cast<decx::_GPU_Matrix<T>*>(&src_);
@@ -484,14 +509,18 @@ DH quantize_f8(GPU_Matrix<T>& src_, GPU_Matrix<uchar>& codes_, GPU_Matrix<S>& sc
     if (!decx_hip_is_init()) return not_init();
     if (!src->Mat.ptr || !src->width || !src->height) return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
     const uint rows = transpose ? src->width : src->height, cols = transpose ? src->height : src->width;
-    DH status = size_output(codes, cols, rows);
-    if (status.error_type == decx::DECX_SUCCESS) status = size_output(scales, block_rows == 128 ? blocks_of_128(rows) : rows, blocks_of_128(cols));
+    F8Output<uchar> q(codes);
+    F8Output<S> s(scales);
+    s.keep_off(src).keep_off(codes);
+    DH status = q.size(cols, rows);
+    if (status.error_type == decx::DECX_SUCCESS) status = s.size(block_rows == 128 ? blocks_of_128(rows) : rows, blocks_of_128(cols));
     if (status.error_type != decx::DECX_SUCCESS) return status;
-    uint8_t* q = codes->Mat.ptr;
-    const int ldq = (int)codes->pitch, lds = (int)scales->pitch;
-    return from_status(decx_hip_f8_quantize(src->Mat.ptr, (int)src->pitch, F8Wide<T>::type, (int)src->height, (int)src->width, block_rows, format,
-                                            F8Scale<S>::type, transpose ? nullptr : q, ldq, transpose ? nullptr : scales->Mat.ptr, lds,
-                                            transpose ? q : nullptr, ldq, transpose ? scales->Mat.ptr : nullptr, lds));
+    const int ldq = (int)q->pitch, lds = (int)s->pitch;
+    const int rc = decx_hip_f8_quantize(src->Mat.ptr, (int)src->pitch, F8Wide<T>::type, (int)src->height, (int)src->width, block_rows, format,
+                                        F8Scale<S>::type, transpose ? nullptr : q->Mat.ptr, ldq, transpose ? nullptr : s->Mat.ptr, lds,
+                                        transpose ? q->Mat.ptr : nullptr, ldq, transpose ? s->Mat.ptr : nullptr, lds);
+    if (rc == 0) s.take_over();
+    return from_status(rc);
 }
 
 template <typename T, typename S>

@@ -1,0 +1,96 @@
+// Calls of the DECX-named 8-bit operators (DECX.h) whose results name a container that the same call reads, is another result,
+// or shares its block with one (operator=): each gives what the same call gives with containers of its own, or is refused.
+// Usage: test_decx_f8_aliases [part] over the fake device (FAKE_DEVICE), test_decx_f8_aliases_gpu [part] over the library's.
+#ifdef FAKE_DEVICE
+#include "fake_device.hpp"
+#endif
+#include <cmath>
+#include <cstdio>
+#include <cstring>
+#include <string>
+#include <type_traits>
+#include <vector>
+
+#include "../../backup_1_amd/host/DECX.h"
+
+static int g_fail = 0;
+#define CHECK(cond)                                                                                          \
+    do {                                                                                                     \
+        if (!(cond)) { std::printf("  CHECK FAILED %s:%d: %s\n", __FILE__, __LINE__, #cond); ++g_fail; }     \
+    } while (0)
+
+template <class T> static T from_float(float v) {
+    if constexpr (std::is_same_v<T, de::Half>) return de::Float2Half(v);
+    else return (T)v;
+}
+// a container of small whole numbers, 1 to 3
+template <class T> static de::GPU_Matrix<T>& filled(uint w, uint h, int seed) {
+    de::Matrix<T>& m = de::CreateMatrixRef<T>(w, h, 0);
+    for (uint i = 0; i < h; ++i)
+        for (uint j = 0; j < w; ++j) m.index((int)i, (int)j) = from_float<T>((float)(1 + (i * 5 + j * 7 + (uint)seed) % 3));
+    de::GPU_Matrix<T>& d = de::CreateGPUMatrixRef<T>(w, h);
+    d.Load_from_host(m);
+    return d;
+}
+template <class T> static de::GPU_Matrix<T>& empty() { return de::CreateGPUMatrixRef<T>(); }
+template <class T> static de::GPU_Matrix<T>& shared(de::GPU_Matrix<T>& of) {
+    de::GPU_Matrix<T>& d = de::CreateGPUMatrixRef<T>();
+    d = of;
+    return d;
+}
+template <class T> static std::vector<T> values(de::GPU_Matrix<T>& d) {
+    de::Matrix<T>& m = de::CreateMatrixRef<T>(d.Width(), d.Height(), 0);
+    d.Load_to_host(m);
+    std::vector<T> v;
+    for (uint i = 0; i < d.Height(); ++i)
+        for (uint j = 0; j < d.Width(); ++j) v.push_back(m.index((int)i, (int)j));
+    return v;
+}
+template <class T> static bool same(de::GPU_Matrix<T>& a, de::GPU_Matrix<T>& b) {
+    if (a.Width() != b.Width() || a.Height() != b.Height()) return false;
+    const std::vector<T> x = values(a), y = values(b);
+    return std::memcmp(x.data(), y.data(), x.size() * sizeof(T)) == 0;
+}
+static bool good(const de::DH& h) { return h.error_type == decx::DECX_SUCCESS; }
+static bool refused(const de::DH& h) { return h.error_type == decx::DECX_FAIL_ErrorParams; }
+
+static void quantize() {
+    for (bool turn : {false, true})
+        for (uint w : {300u, 1u}) {
+            auto call = [&](auto& src, auto& codes, auto& scales) {
+                return turn ? de::cuda::Quantize_f8_T(src, codes, scales, 1, 0) : de::cuda::Quantize_f8(src, codes, scales, 1, 0);
+            };
+            de::GPU_Matrix<float>&src = filled<float>(w, w == 1 ? 1 : 5, 1), &scales = empty<float>();
+            de::GPU_Matrix<uchar>& codes = empty<uchar>();
+            CHECK(good(call(src, codes, scales)));
+            for (bool handle : {false, true}) {
+                de::GPU_Matrix<float>& x = filled<float>(w, w == 1 ? 1 : 5, 1);
+                de::GPU_Matrix<float>& s = handle ? shared(x) : x;
+                de::GPU_Matrix<uchar>& c = empty<uchar>();
+                CHECK(good(call(x, c, s)) && same(c, codes) && same(s, scales));
+                CHECK(!handle || same(x, src));
+            }
+            // results on one block: 1 x 1 is the size for which neither is made anew
+            de::GPU_Matrix<uchar>&c = filled<uchar>(1, 1, 0), &s = shared(c), &want_c = empty<uchar>(), &want_s = empty<uchar>();
+            CHECK(good(call(src, want_c, want_s)) && good(call(src, c, s)) && same(c, want_c) && same(s, want_s));
+            CHECK(refused(call(src, c, c)));
+        }
+}
+
+int main(int argc, char** argv) {
+    const std::string only = argc > 1 ? argv[1] : "";
+    de::InitCuda();
+    struct { const char* name; void (*run)(); } parts[] = {{"quantize", quantize}};
+    for (auto& part : parts) {
+        if (!only.empty() && only != part.name) continue;
+        const int before = g_fail;
+        part.run();
+#ifdef FAKE_DEVICE
+        CHECK(fake::faults == 0 && fake::calls > 0);
+        fake::faults = fake::calls = 0;
+#endif
+        std::printf("%s: %d failure(s)\n", part.name, g_fail - before);
+        std::fflush(stdout);
+    }
+    return g_fail ? 1 : 0;
+}
