@@ -537,11 +537,15 @@ DH gemm_f8(GPU_Matrix<uchar>& A_, GPU_Matrix<S>& sA_, int fA, GPU_Matrix<uchar>&
     const bool by_rows = sB->width == N, by_blocks = sB->width == blocks_of_128(N);
     if (B->width != K || sA->width != M || sA->height != blocks_of_128(K) || sB->height != blocks_of_128(K) || !(by_rows || by_blocks))
         return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
-    const DH status = size_output(dst, N, M);
+    F8Output<T> out(dst);
+    out.keep_off(sA).keep_off(sB);
+    const DH status = out.size(N, M);
     if (status.error_type != decx::DECX_SUCCESS) return status;
-    return from_status(decx_hip_f8gemm(A->Mat.ptr, (int)A->pitch, fA, sA->Mat.ptr, (int)sA->pitch, B->Mat.ptr, (int)B->pitch, fB, sB->Mat.ptr,
-                                       (int)sB->pitch, by_rows ? 1 : 128, F8Scale<S>::type, nullptr, 0, dst->Mat.ptr, (int)dst->pitch,
-                                       F8Wide<T>::type, (int)M, (int)N, (int)K));
+    const int rc = decx_hip_f8gemm(A->Mat.ptr, (int)A->pitch, fA, sA->Mat.ptr, (int)sA->pitch, B->Mat.ptr, (int)B->pitch, fB, sB->Mat.ptr,
+                                   (int)sB->pitch, by_rows ? 1 : 128, F8Scale<S>::type, nullptr, 0, out->Mat.ptr, (int)out->pitch,
+                                   F8Wide<T>::type, (int)M, (int)N, (int)K);
+    if (rc == 0) out.take_over();
+    return from_status(rc);
 }
 
 template <typename T>

@@ -77,10 +77,33 @@ static void quantize() {
         }
 }
 
+// dst over either operand's scales; M = 1 and N = 1 leave a scales' container its size for some K
+static void gemm() {
+    for (uint M : {1u, 3u})
+        for (uint N : {1u, 40u})
+            for (uint K : {100u, 300u}) {
+                const uint kb = (K + 127) / 128;
+                de::GPU_Matrix<uchar>&a = filled<uchar>(K, M, 1), &b = filled<uchar>(K, N, 2);
+                de::GPU_Matrix<float>&sa = filled<float>(M, kb, 3), &sb = filled<float>(N, kb, 4), &want = empty<float>();
+                CHECK(good(de::cuda::GEMM_f8(a, sa, 0, b, sb, 0, want)) && want.Width() == N && want.Height() == M);
+                for (int which : {0, 1, 2, 3}) {
+                    de::GPU_Matrix<float>&pa = filled<float>(M, kb, 3), &pb = filled<float>(N, kb, 4);
+                    de::GPU_Matrix<float>& over = which & 1 ? pb : pa;
+                    de::GPU_Matrix<float>& dst = which & 2 ? shared(over) : over;
+                    CHECK(good(de::cuda::GEMM_f8(a, pa, 0, b, pb, 0, dst)) && same(dst, want));
+                    CHECK(which != 2 || (same(pa, sa) && same(pb, sb)));
+                    CHECK(which != 3 || (same(pa, sa) && same(pb, sb)));
+                }
+                de::GPU_Matrix<float>& s1 = filled<float>(M, kb, 3);
+                de::GPU_Matrix<uchar>& b1 = filled<uchar>(K, M, 2);              // one container scales both operands and takes the result
+                CHECK(good(de::cuda::GEMM_f8(a, s1, 0, b1, s1, 0, s1)) && s1.Width() == M && s1.Height() == M);
+            }
+}
+
 int main(int argc, char** argv) {
     const std::string only = argc > 1 ? argv[1] : "";
     de::InitCuda();
-    struct { const char* name; void (*run)(); } parts[] = {{"quantize", quantize}};
+    struct { const char* name; void (*run)(); } parts[] = {{"quantize", quantize}, {"gemm", gemm}};
     for (auto& part : parts) {
         if (!only.empty() && only != part.name) continue;
         const int before = g_fail;
