@@ -16,6 +16,7 @@ namespace {
 char kSuccess[] = "No error\n";                                              // core/error.h:61
 char kGemmDims[] = "The width of matrix A and the height of matrix B are required to be same";   // core/error.h GEMM_DimNMatch
 char kMDims[] = "Matrix Dims don't match each other";
+char kOneContainer[] = "One container cannot be two results\n";
 char kNotFactory[] = "Container was not created by this library's factories\n";
 
 de::DH ok() { return de::DH{decx::DECX_SUCCESS, kSuccess}; }
@@ -563,14 +564,24 @@ DH rmsnorm_f8(GPU_Matrix<T>& src_, GPU_Matrix<T>& residual_, GPU_Matrix<T>& weig
     const uint M = src->height, K = src->width;
     if (!src->Mat.ptr || !residual->Mat.ptr || !weight->Mat.ptr || !M || !K || residual->width != K || residual->height != M || weight->width != K)
         return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
-    DH status = size_output(sum, K, M);
-    if (status.error_type == decx::DECX_SUCCESS) status = size_output(rstd, M, 1);
-    if (status.error_type == decx::DECX_SUCCESS) status = size_output(codes, K, M);
-    if (status.error_type == decx::DECX_SUCCESS) status = size_output(scales, M, blocks_of_128(K));
+    if constexpr (std::is_same_v<T, float>)
+        if (sum == rstd || sum == scales) return DH{decx::DECX_FAIL_ErrorParams, kOneContainer};
+    F8Output<T> h(sum);                                         // over src or residual in place
+    F8Output<float> r(rstd), s(scales);
+    F8Output<uchar> q(codes);
+    h.keep_off(weight);
+    r.keep_off(src).keep_off(residual).keep_off(weight).keep_off(sum);
+    s.keep_off(src).keep_off(residual).keep_off(weight).keep_off(sum).keep_off(rstd);
+    DH status = h.size(K, M);
+    if (status.error_type == decx::DECX_SUCCESS) status = r.size(M, 1);
+    if (status.error_type == decx::DECX_SUCCESS) status = q.size(K, M);
+    if (status.error_type == decx::DECX_SUCCESS) status = s.size(M, blocks_of_128(K));
     if (status.error_type != decx::DECX_SUCCESS) return status;
-    return from_status(decx_hip_rmsnorm_f8(src->Mat.ptr, (int)src->pitch, residual->Mat.ptr, (int)residual->pitch, weight->Mat.ptr, eps,
-                                           F8Wide<T>::type, (int)M, (int)K, sum->Mat.ptr, (int)sum->pitch, rstd->Mat.ptr, nullptr, 0,
-                                           codes->Mat.ptr, (int)codes->pitch, scales->Mat.ptr, (int)scales->pitch, format, DECX_HIP_SCALE_F32));
+    const int rc = decx_hip_rmsnorm_f8(src->Mat.ptr, (int)src->pitch, residual->Mat.ptr, (int)residual->pitch, weight->Mat.ptr, eps,
+                                       F8Wide<T>::type, (int)M, (int)K, h->Mat.ptr, (int)h->pitch, r->Mat.ptr, nullptr, 0, q->Mat.ptr,
+                                       (int)q->pitch, s->Mat.ptr, (int)s->pitch, format, DECX_HIP_SCALE_F32);
+    if (rc == 0) h.take_over(), r.take_over(), s.take_over();
+    return from_status(rc);
 }
 
 template <typename T>

@@ -100,10 +100,62 @@ static void gemm() {
             }
 }
 
+template <class T> struct NormCase {
+    de::GPU_Matrix<T>&src, &residual, &weight, *sum;
+    de::GPU_Matrix<float>*rstd, *scales;
+    de::GPU_Matrix<uchar>& codes;
+    NormCase(uint M, uint K)
+        : src(filled<T>(K, M, 1)), residual(filled<T>(K, M, 2)), weight(filled<T>(K, 1, 3)), sum(&empty<T>()), rstd(&empty<float>()),
+          scales(&empty<float>()), codes(empty<uchar>()) {}
+    de::DH run() { return de::nn::RMSNorm_f8(src, residual, weight, 0.5f, *sum, *rstd, codes, *scales, 0); }
+    bool as(NormCase& o) { return same(*sum, *o.sum) && same(*rstd, *o.rstd) && same(codes, o.codes) && same(*scales, *o.scales); }
+};
+template <class T> static void norm() {
+    for (uint M : {1u, 4u})
+        for (uint K : {1u, 4u, 300u}) {
+            NormCase<T> plain(M, K);
+            CHECK(good(plain.run()));
+            for (bool handle : {false, true}) {
+                for (int which : {0, 1, 2}) {                                  // the sum over src, residual (in place), weight
+                    NormCase<T> c(M, K);
+                    de::GPU_Matrix<T>& over = which == 0 ? c.src : which == 1 ? c.residual : c.weight;
+                    c.sum = handle ? &shared(over) : &over;
+                    CHECK(good(c.run()) && c.as(plain));
+                    CHECK(which != 2 || !handle || same(c.weight, plain.weight));
+                }
+                if constexpr (std::is_same_v<T, float>)
+                    for (int result : {0, 1})                                  // rstd, the scales over each of the matrices
+                        for (int which : {0, 1, 2}) {
+                            NormCase<T> c(M, K);
+                            de::GPU_Matrix<T>& over = which == 0 ? c.src : which == 1 ? c.residual : c.weight;
+                            (result ? c.scales : c.rstd) = handle ? &shared(over) : &over;
+                            CHECK(good(c.run()) && c.as(plain));
+                            CHECK(!handle || same(over, which == 0 ? plain.src : which == 1 ? plain.residual : plain.weight));
+                        }
+            }
+            if constexpr (std::is_same_v<T, float>) {
+                for (int which : {0, 1}) {                                     // two results of one container, or on one block
+                    NormCase<T> c(M, K), d(M, K);
+                    (which ? c.scales : c.rstd) = c.sum;
+                    CHECK(refused(c.run()));
+                    d.sum = &filled<float>(K, M, 5);
+                    (which ? d.scales : d.rstd) = &shared(*d.sum);
+                    CHECK(good(d.run()) && d.as(plain));
+                }
+            }
+            NormCase<T> c(M, K), d(M, K);
+            c.scales = c.rstd;
+            CHECK(refused(c.run()));
+            d.rstd = &filled<float>(M, 1, 5);
+            d.scales = &shared(*d.rstd);
+            CHECK(good(d.run()) && d.as(plain));
+        }
+}
+
 int main(int argc, char** argv) {
     const std::string only = argc > 1 ? argv[1] : "";
     de::InitCuda();
-    struct { const char* name; void (*run)(); } parts[] = {{"quantize", quantize}, {"gemm", gemm}};
+    struct { const char* name; void (*run)(); } parts[] = {{"quantize", quantize}, {"gemm", gemm}, {"norm", [] { norm<float>(); norm<de::Half>(); }}};
     for (auto& part : parts) {
         if (!only.empty() && only != part.name) continue;
         const int before = g_fail;
