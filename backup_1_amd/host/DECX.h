@@ -275,7 +275,8 @@ DH ReLU_f_Rec(GPU_Matrix<float>& src, GPU_Matrix<float>& dst, GPU_Matrix<uchar>&
 DH ReLU_f_Backward(GPU_Matrix<float>& src, GPU_Matrix<float>& dst, GPU_Matrix<uchar>& rec_map);
 // Root-mean-square norm of the rows of src + residual with its result as 8-bit codes scaled by rows (decx_hip_rmsnorm_f8), and
 // its gradient (decx_hip_rmsnorm_backward).  weight is one row; sum (which may be src or residual), codes, scales and rstd (one
-// row, a factor for each row of src) are sized as needed; grad_weight becomes one row.  dst may be grad.
+// row, a factor for each row of src) are sized as needed; grad_weight becomes one row.  dst may be grad or sum.
+// Other results over inputs: as the products'.
 DH RMSNorm_f8(GPU_Matrix<float>& src, GPU_Matrix<float>& residual, GPU_Matrix<float>& weight, const float eps, GPU_Matrix<float>& sum,
               GPU_Matrix<float>& rstd, GPU_Matrix<uchar>& codes, GPU_Matrix<float>& scales, const int format);
 DH RMSNorm_f8(GPU_Matrix<Half>& src, GPU_Matrix<Half>& residual, GPU_Matrix<Half>& weight, const float eps, GPU_Matrix<Half>& sum,

@@ -600,15 +600,23 @@ DH rmsnorm_f8_backward(GPU_Matrix<T>& sum_, GPU_Matrix<T>& weight_, GPU_Matrix<f
     if (!sum->Mat.ptr || !weight->Mat.ptr || !rstd->Mat.ptr || !grad->Mat.ptr || !M || !K || weight->width != K || rstd->width != M ||
         grad->width != K || grad->height != M)
         return DH{decx::DECX_FAIL_DimsNotMatching, kMDims};
-    DH status = size_output(dst, K, M);
-    if (status.error_type == decx::DECX_SUCCESS) status = size_output(grad_weight, K, 1);
+    if constexpr (std::is_same_v<T, float>)
+        if (dst == grad_weight) return DH{decx::DECX_FAIL_ErrorParams, kOneContainer};
+    F8Output<T> dx(dst);                                        // over grad or sum in place
+    F8Output<float> dw(grad_weight);
+    dx.keep_off(weight).keep_off(rstd);
+    dw.keep_off(sum).keep_off(weight).keep_off(grad).keep_off(dst);
+    DH status = dx.size(K, M);
+    if (status.error_type == decx::DECX_SUCCESS) status = dw.size(K, 1);
     if (status.error_type != decx::DECX_SUCCESS) return status;
     DeviceTemp work;
     const size_t bytes = decx_hip_rmsnorm_backward_workspace((int)M, (int)K);
     if (int rc = work.alloc(bytes)) return rc == DECX_HIP_FAIL_ALLOCATION ? alloc_fail() : from_status(rc);
-    return from_status(decx_hip_rmsnorm_backward(sum->Mat.ptr, (int)sum->pitch, weight->Mat.ptr, rstd->Mat.ptr, grad->Mat.ptr, (int)grad->pitch,
-                                                 nullptr, 0, F8Wide<T>::type, (int)M, (int)K, dst->Mat.ptr, (int)dst->pitch,
-                                                 grad_weight->Mat.ptr, work.ptr, bytes));
+    const int rc = decx_hip_rmsnorm_backward(sum->Mat.ptr, (int)sum->pitch, weight->Mat.ptr, rstd->Mat.ptr, grad->Mat.ptr, (int)grad->pitch,
+                                             nullptr, 0, F8Wide<T>::type, (int)M, (int)K, dx->Mat.ptr, (int)dx->pitch, dw->Mat.ptr, work.ptr,
+                                             bytes);
+    if (rc == 0) dx.take_over(), dw.take_over();
+    return from_status(rc);
 }
 }  // namespace
 

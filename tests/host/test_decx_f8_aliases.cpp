@@ -152,10 +152,66 @@ template <class T> static void norm() {
         }
 }
 
+template <class T> struct BackwardCase {
+    de::GPU_Matrix<T>&sum, &weight, &grad, *dst;
+    de::GPU_Matrix<float>&rstd, *grad_weight;
+    BackwardCase(uint M, uint K)
+        : sum(filled<T>(K, M, 1)), weight(filled<T>(K, 1, 2)), grad(filled<T>(K, M, 3)), dst(&empty<T>()), rstd(filled<float>(M, 1, 4)),
+          grad_weight(&empty<float>()) {}
+    de::DH run() { return de::nn::RMSNorm_f8_Backward(sum, weight, rstd, grad, *dst, *grad_weight); }
+    // dst bit for bit; dW's parts may be added in another order where dst lies over an input: whole numbers, so the same but for rstd's
+    bool as(BackwardCase& o) {
+        const std::vector<float> x = values(*grad_weight), y = values(*o.grad_weight);
+        bool near = x.size() == y.size();
+        for (size_t i = 0; near && i < x.size(); ++i) near = std::fabs(x[i] - y[i]) <= 1e-6f * std::fabs(y[i]);
+        return same(*dst, *o.dst) && near;
+    }
+};
+template <class T> static void backward() {
+    for (uint M : {1u, 4u})
+        for (uint K : {1u, 4u, 300u}) {
+            BackwardCase<T> plain(M, K);
+            CHECK(good(plain.run()));
+            for (bool handle : {false, true}) {
+                for (int which : {0, 1, 2}) {                                  // dst over grad, sum (in place), weight
+                    BackwardCase<T> c(M, K);
+                    de::GPU_Matrix<T>& over = which == 0 ? c.grad : which == 1 ? c.sum : c.weight;
+                    c.dst = handle ? &shared(over) : &over;
+                    CHECK(good(c.run()) && c.as(plain));
+                    CHECK(which != 2 || !handle || same(c.weight, plain.weight));
+                }
+                BackwardCase<T> r(M, K);
+                r.grad_weight = handle ? &shared(r.rstd) : &r.rstd;
+                CHECK(refused(r.run()));
+                if constexpr (std::is_same_v<T, float>) {
+                    BackwardCase<T> d(M, K);
+                    d.dst = handle ? &shared(d.rstd) : &d.rstd;
+                    CHECK(good(d.run()) && d.as(plain));
+                    for (int which : {0, 1, 2}) {                              // the weight's gradient over each of the matrices
+                        BackwardCase<T> c(M, K);
+                        de::GPU_Matrix<T>& over = which == 0 ? c.grad : which == 1 ? c.sum : c.weight;
+                        c.grad_weight = handle ? &shared(over) : &over;
+                        CHECK(good(c.run()) && c.as(plain));
+                        CHECK(!handle || same(over, which == 0 ? plain.grad : which == 1 ? plain.sum : plain.weight));
+                    }
+                }
+            }
+            if constexpr (std::is_same_v<T, float>) {
+                BackwardCase<T> c(M, K), d(M, K);
+                c.grad_weight = c.dst;
+                CHECK(refused(c.run()));
+                d.dst = &filled<float>(K, M, 5);
+                d.grad_weight = &shared(*d.dst);
+                CHECK(good(d.run()) && d.as(plain));
+            }
+        }
+}
+
 int main(int argc, char** argv) {
     const std::string only = argc > 1 ? argv[1] : "";
     de::InitCuda();
-    struct { const char* name; void (*run)(); } parts[] = {{"quantize", quantize}, {"gemm", gemm}, {"norm", [] { norm<float>(); norm<de::Half>(); }}};
+    struct { const char* name; void (*run)(); } parts[] = {{"quantize", quantize}, {"gemm", gemm}, {"norm", [] { norm<float>(); norm<de::Half>(); }},
+                                                           {"backward", [] { backward<float>(); backward<de::Half>(); }}};
     for (auto& part : parts) {
         if (!only.empty() && only != part.name) continue;
         const int before = g_fail;

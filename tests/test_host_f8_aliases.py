@@ -6,7 +6,7 @@ import subprocess
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-PARTS = ("quantize", "gemm", "norm")
+PARTS = ("quantize", "gemm", "norm", "backward")
 
 
 def _run(name, part):
