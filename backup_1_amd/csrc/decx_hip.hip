@@ -80,6 +80,11 @@ int check_element_alignment(const void* p, int type) {
     return 0;
 }
 
+int check_results(std::initializer_list<Result> results, std::initializer_list<Operand> inputs) {
+    if (results_fit(results, inputs)) return 0;
+    return fail(DECX_HIP_FAIL_ERROR_PARAMS, "a result lies over an input, or over another result\n");
+}
+
 // the fp32 workspace of the fp16 split-K paths: reserved by decx_hip_init for every split the library chooses by itself
 // (at most one 128x128 tile and range per CU, twice that in the atomic mode's tile count), grown only for larger forced
 // splits, kept until the process ends

@@ -244,6 +244,11 @@ int f8_quantize_enqueue(const void* X, int ldx, int type, int M, int K, int bloc
     if (int rc = check_element_alignment(X, type)) return rc;
     if (scale_type == DECX_HIP_SCALE_F32 && ((reinterpret_cast<uintptr_t>(Q ? S : nullptr) | reinterpret_cast<uintptr_t>(Qt ? St : nullptr)) & 3u))
         return fail(DECX_HIP_FAIL_ERROR_PARAMS, "scales off the grid of their type\n");
+    const size_t m = (size_t)M, k = (size_t)K, one = scale_size(scale_type);
+    if (int rc = check_results({{operand(Q, m, k, ldq, 1)}, {operand(Q ? S : nullptr, cdiv(K, kScaleBlock), row_scales, lds, one)},
+                                {operand(Qt, k, m, ldqt, 1)}, {operand(Qt ? St : nullptr, cdiv(M, kScaleBlock), col_scales, ldst, one)}},
+                               {operand(X, m, k, ldx, element_size(type))}))
+        return rc;
     const int e5m2 = format == DECX_HIP_E5M2, e8m0 = scale_type == DECX_HIP_SCALE_E8M0;
     if (type == DECX_HIP_F32) return f8_quantize_launch<0>(X, ldx, M, K, block_rows, e5m2, e8m0, Q, ldq, S, lds, Qt, ldqt, St, ldst);
     if (type == DECX_HIP_F16) return f8_quantize_launch<1>(X, ldx, M, K, block_rows, e5m2, e8m0, Q, ldq, S, lds, Qt, ldqt, St, ldst);

@@ -75,6 +75,11 @@ int f8gemm_enqueue(const uint8_t* A, int lda, int format_a, const void* SA, int 
     if (int rc = check_element_alignment(Cin, type)) return rc;
     if (scale_type == DECX_HIP_SCALE_F32 && ((reinterpret_cast<uintptr_t>(SA) | reinterpret_cast<uintptr_t>(SB)) & 3u))
         return fail(DECX_HIP_FAIL_ERROR_PARAMS, "scales off the grid of their type\n");
+    const size_t m = (size_t)M, n = (size_t)N, k = (size_t)K, wide = element_size(type), one = scale_size(scale_type), blocks = cdiv(K, kScaleBlock);
+    if (int rc = check_results({{operand(D, m, n, ldd, wide), 1u}},
+                               {operand(Cin, m, n, ldc, wide), operand(A, m, k, lda, 1), operand(B, n, k, ldb, 1), operand(SA, blocks, m, ldsa, one),
+                                operand(SB, blocks, b_block_rows == 1 ? N : cdiv(N, kScaleBlock), ldsb, one)}))
+        return rc;
     F8GemmArgs g = {};
     g.A = A, g.B = B, g.SA = SA, g.SB = SB, g.C = Cin, g.D = D;
     g.lda = (size_t)lda, g.ldb = (size_t)ldb, g.ldsa = (size_t)ldsa, g.ldsb = (size_t)ldsb, g.ldc = (size_t)ldc, g.ldd = (size_t)ldd;

@@ -423,6 +423,12 @@ int rmsnorm_f8_enqueue(const void* X, int ldx, const void* R, int ldr, const voi
     if (int rc = check_element_alignment(rstd, DECX_HIP_F32)) return rc;
     if (Q && scale_type == DECX_HIP_SCALE_F32 && (reinterpret_cast<uintptr_t>(S) & 3u))
         return fail(DECX_HIP_FAIL_ERROR_PARAMS, "scales off the grid of their type\n");
+    // a thread reads its elements of a row before it writes them, so H or Y may lie over X or R
+    const size_t m = (size_t)M, k = (size_t)K, wide = element_size(type);
+    if (int rc = check_results({{operand(H, m, k, ldh, wide), 3u}, {operand(Y, m, k, ldy, wide), 3u}, {operand(rstd, 1, m, m, 4)}, {operand(Q, m, k, ldq, 1)},
+                                {operand(Q ? S : nullptr, cdiv(K, kScaleBlock), m, lds, scale_size(scale_type))}},
+                               {operand(X, m, k, ldx, wide), operand(R, m, k, ldr, wide), operand(W, 1, k, k, wide)}))
+        return rc;
     RmsNormArgs g = {};
     g.X = X, g.R = R, g.W = W, g.H = H, g.Y = Y, g.rstd = rstd, g.Q = Q, g.S = S;
     g.ldx = (size_t)ldx, g.ldr = (size_t)ldr, g.ldh = (size_t)ldh, g.ldy = (size_t)ldy, g.ldq = (size_t)ldq, g.lds = (size_t)lds;
@@ -469,6 +475,11 @@ int rmsnorm_backward_enqueue(const void* H, int ldh, const void* W, const float*
     if (dW && (!work || (reinterpret_cast<uintptr_t>(work) & 3u) || work_bytes < rmsnorm_backward_workspace(M, K)))
         return fail(DECX_HIP_FAIL_ERROR_PARAMS, "the weight's gradient needs a workspace of %zu bytes (decx_hip_rmsnorm_backward_workspace)\n",
                     rmsnorm_backward_workspace(M, K));
+    const size_t m = (size_t)M, k = (size_t)K, wide = element_size(type), need = rmsnorm_backward_workspace(M, K);
+    if (int rc = check_results({{operand(dX, m, k, lddx, wide), 7u}, {operand(dW, 1, k, k, 4)}, {operand(dW ? work : nullptr, 1, need, need, 1)}},
+                               {operand(H, m, k, ldh, wide), operand(dY, m, k, lddy, wide), operand(dR, m, k, lddr, wide), operand(W, 1, k, k, wide),
+                                operand(rstd, 1, m, m, 4)}))
+        return rc;
     const int groups = rmsnorm_backward_groups(M, K, type == DECX_HIP_F32 ? 4 : 2);
     RmsNormBackwardArgs g = {};
     g.H = H, g.W = W, g.dY = dY, g.dR = dR, g.rstd = rstd, g.dX = dX, g.row_groups = groups;

@@ -8,6 +8,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "operands.hpp"
+
 namespace decx_hip {
 
 struct Runtime {
@@ -78,6 +80,11 @@ int need_library_device();
 int check_f8_codes(int type, int format, int scale_type);
 // a matrix must lie on the grid of its own elements (nullptr does)
 int check_element_alignment(const void* p, int type);
+
+// refuses results that meet an input or each other (operands.hpp): what a workgroup reads another would write
+int check_results(std::initializer_list<Result> results, std::initializer_list<Operand> inputs);
+inline size_t element_size(int type) { return type == DECX_HIP_F32 ? 4 : 2; }
+inline size_t scale_size(int scale_type) { return scale_type == DECX_HIP_SCALE_F32 ? 4 : 1; }
 
 // zero-fills the M x N region of a pitched matrix on `stream` (the split-K kernels accumulate into it)
 void enqueue_zero_region(float* D, int ldd, int M, int N, hipStream_t stream);

@@ -247,6 +247,8 @@ int decx_hip_relu_f32_backward(const float* src, float* dst, const unsigned char
  * family in the same manner: the same conventions, error codes, library stream, and _async forms.  They take no workspace
  * of the library and allocate nothing, so any of them may be captured into a graph, and graphs and calls that share no
  * result (or caller's workspace) may overlap.  The calling thread's current device must be the one decx_hip_init saw.
+ * A result may lie over an input where its call says so, at that input's pitch, and may otherwise meet no input and no other
+ * result (columns of one matrix do not): such calls are refused.
  * Matrices may lie at any address that is a multiple of their element's size, with any pitch; D, Q, H, Y and dX are
  * written within their rows only; of what lies beyond a row's K (N) elements at most the rest of the aligned 16 bytes that
  * hold the last one is read, and not used.  Sizes are at least 1. */
@@ -307,8 +309,8 @@ int decx_hip_f8gemm_plan(int M, int N, int K, int type, int scale_type, int b_bl
 
 /* Root-mean-square norm of the rows of X + R (R nullable: of X), K <= 32768:
  *   h = x + r rounded to `type`;  rstd = 1 / sqrt(mean of h^2 over the row + eps);  y = h * rstd * w
- * Results, each nullable but not all: H (may be X or R itself, at its pitch), rstd (M floats; what the gradient needs), Y in
- * `type`, and Q, S: y -- in fp32, not rounded to `type` before -- as decx_hip_f8_quantize gives it with block_rows = 1.
+ * Results, each nullable but not all: H and Y in `type` (each may be X or R itself, at its pitch), rstd (M floats; what the
+ * gradient needs), and Q, S: y -- in fp32, not rounded to `type` before -- as decx_hip_f8_quantize gives it with block_rows = 1.
  * W holds K elements of `type`.  Sums are in fp32. */
 int decx_hip_rmsnorm_f8(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H, int ldh,
                         float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type);
@@ -320,7 +322,7 @@ int decx_hip_rmsnorm_f8_async(const void* X, int ldx, const void* R, int ldr, co
  *                                                              through H itself; dX may be dY, dR or H at its pitch)
  *   dW[k] = sum over the rows of dy * n                       (K floats; nullable)
  * dW takes a workspace of the caller of decx_hip_rmsnorm_backward_workspace(M, K) bytes, 4-byte aligned, which need not be
- * cleared and must not be shared by calls that overlap; the rows' parts are added in order, the same bits on every run. */
+ * cleared, meets no other operand and must not be shared by calls that overlap; the rows' parts are added in order, the same bits on every run. */
 size_t decx_hip_rmsnorm_backward_workspace(int M, int K);
 int decx_hip_rmsnorm_backward(const void* H, int ldh, const void* W, const float* rstd, const void* dY, int lddy, const void* dR, int lddr,
                               int type, int M, int K, void* dX, int lddx, float* dW, void* work, size_t work_bytes);
