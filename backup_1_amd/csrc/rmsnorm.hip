@@ -14,8 +14,8 @@
 namespace decx_hip {
 
 // Sum over the workgroup, in every thread.  `part` is used by one call at a time: the callers separate calls by a barrier.
-template <int NT>
-__device__ __forceinline__ float workgroup_sum(float v, float* part) {
+template <int NT, class T>
+__device__ __forceinline__ T workgroup_sum(T v, T* part) {
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d);
     if constexpr (NT > kWave) {
@@ -35,6 +35,11 @@ __device__ __forceinline__ int xcd_row(int pid, int rows) {
     return xcd * base + (xcd < rem ? xcd : rem) + local;
 }
 
+// Squares of elements beyond 2^64 overflow fp32, those of elements below 2^-63 lose bits.  Where the mean of a row is infinite, or
+// so small that lost bits could matter (each square at most 2^-150, half of fp32's smallest step), its squares are added again in
+// 64 bits from the registers.
+constexpr float kLeastMean = 0x1p-120f;
+
 struct RmsNormArgs {
     const void *X, *R, *W;
     void *H, *Y;
@@ -50,6 +55,7 @@ template <int TYPE, int NT, int CH, int ROWS>
 __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
     typedef typename Wide<TYPE>::T T;
     __shared__ float part[NT / kWave];
+    __shared__ double part64[NT / kWave];
     const int K = g.K, m = xcd_row((int)blockIdx.x, g.M);
     const T* x = static_cast<const T*>(g.X) + (size_t)m * g.ldx;
     Eight h[CH];
@@ -90,7 +96,18 @@ __global__ __launch_bounds__(NT) void rmsnorm_f8_kernel(const RmsNormArgs g) {
             store8_part<TYPE>(static_cast<T*>(g.H) + (size_t)m * g.ldh + (k < K ? k : 0), h[i], K - k);
         }
     }
-    const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(workgroup_sum<NT>(sum, part), (float)K) + g.eps));
+    const float mean = __fdiv_rn(workgroup_sum<NT>(sum, part), (float)K) + g.eps;
+    float rstd;
+    if (mean >= kLeastMean && mean < __builtin_inff()) {        // the same for the whole workgroup
+        rstd = __fdiv_rn(1.f, __fsqrt_rn(mean));
+    } else {
+        double squares = 0.0;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) squares += (double)h[i].v[e] * h[i].v[e];
+        rstd = (float)(1.0 / sqrt(workgroup_sum<NT>(squares, part64) / K + (double)g.eps));
+    }
     if (g.rstd && threadIdx.x == 0) g.rstd[m] = rstd;
     if (!g.Q && !g.Y) return;
 #pragma unroll

@@ -311,7 +311,8 @@ int decx_hip_f8gemm_plan(int M, int N, int K, int type, int scale_type, int b_bl
  *   h = x + r rounded to `type`;  rstd = 1 / sqrt(mean of h^2 over the row + eps);  y = h * rstd * w
  * Results, each nullable but not all: H and Y in `type` (each may be X or R itself, at its pitch), rstd (M floats; what the
  * gradient needs), and Q, S: y -- in fp32, not rounded to `type` before -- as decx_hip_f8_quantize gives it with block_rows = 1.
- * W holds K elements of `type`.  Sums are in fp32. */
+ * W holds K elements of `type`.  Sums are in fp32, those of rows whose squares leave its range in 64 bits; rstd is an fp32
+ * number, and so infinite where sqrt(mean of h^2 + eps) is below 2^-128. */
 int decx_hip_rmsnorm_f8(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H, int ldh,
                         float* rstd, void* Y, int ldy, uint8_t* Q, int ldq, void* S, int lds, int format, int scale_type);
 int decx_hip_rmsnorm_f8_async(const void* X, int ldx, const void* R, int ldr, const void* W, float eps, int type, int M, int K, void* H,

@@ -321,3 +321,29 @@ def test_inputs_larger_than_the_caches(gpu, kind, M, K, times):
     assert np.array_equal(dx.view(np.uint8), big(dx[:M]).view(np.uint8))
     _, _, want_w, size_w = gradient64(ref.from_type(x, kind), ref.from_type(w, kind), rstd.astype(np.float64), ref.from_type(r, kind), 0.0)
     assert np.all(np.abs(dw - times * want_w) <= times * size_w * (times * M + 20) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("kind", [capi.F32, capi.BF16], ids=lambda k: ref.TYPE_NAMES[k])
+@pytest.mark.parametrize("power,eps", [(70, EPS), (122, EPS), (64, 0.0), (63, EPS), (-64, 0.0), (-80, 0.0), (-110, 0.0), (-80, EPS), (-61, 1e-37)])
+@pytest.mark.parametrize("M,K", [(3, 7), (4, 300), (3, 1500), (2, 4100), (2, 9000), (2, 20000)])
+def test_rows_whose_squares_leave_fp32(gpu, kind, power, eps, M, K):
+    """Finite rows whose squares overflow or lose their bits, beside an ordinary row: the bounds are those of ordinary rows."""
+    x, r = (workloads.normal((M, K), s).astype(np.float32) * np.float32(2.0 ** power) for s in (50, 51))
+    x[0], r[0] = workloads.normal((K,), 52), 0
+    x, r, w = ref.to_type(x, kind), ref.to_type(r, kind), ref.to_type(1 + 0.2 * workloads.normal((1, K), 53), kind)
+    got = run(x, r, w, kind, eps=eps)
+    check(x, r, w, kind, got, eps=eps)
+    if abs(power) <= 80:                                         # the gradient by that rstd; beyond, dx leaves the types' normal range
+        dy = ref.to_type(workloads.normal((M, K), 54), kind)
+        check_backward(got["H"], w, got["rstd"][0], dy, None, kind, backward(got["H"], w, got["rstd"][0], dy, None, kind), M)
+
+
+def test_rows_at_the_ends_of_fp32(gpu):
+    """Rows of the largest finite values, whose rstd is subnormal (half its step is 2^-22 of it, within the bounds); rows whose
+    rstd no fp32 holds."""
+    x = np.where(workloads.normal((2, 600), 55) > 0, np.float32(3e38), np.float32(-2e38)).astype(np.float32)
+    w = np.ones((1, 600), np.float32)
+    got = run(x, None, w, capi.F32, eps=0.0)
+    check(x, None, w, capi.F32, got, eps=0.0)
+    least = run(np.full((1, 600), 1e-44, np.float32), None, w, capi.F32, eps=0.0)
+    assert np.all(np.isinf(least["rstd"]))
