@@ -277,3 +277,79 @@ def test_plain_and_packed_entry_points_agree(gpu):
             capi.sync()
     for a, c in zip(p, o):
         assert np.array_equal(a.result().view(np.uint8), c.result().view(np.uint8))
+
+
+# what every kernel takes: kernel 6 no fp32 scale for each row of B
+KINDS_OF_SCALE = [(capi.SCALE_F32, 1), (capi.SCALE_F32, 128), (capi.SCALE_E8M0, 1), (capi.SCALE_E8M0, 128)]
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("scale,b_rows", KINDS_OF_SCALE)
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+def test_nan_by_every_kernel(forced, variant, scale, b_rows, kind):
+    """A NaN code or scale of A in its row, of B in its column (or its 128), and all other results in their clean bits."""
+    forced(variant)
+    for M, N, K in ((5, 40, 272), (300, 530, 400)):
+        a, sa = real_operand(M, K, capi.E4M3, scale, 1, 41)
+        b, sb = real_operand(N, K, capi.E5M2, scale, b_rows, 42)
+        args = (capi.E4M3, b_rows, kind)
+        clean = run(a, sa, args[0], b, sb, capi.E5M2, *args[1:]).view(np.uint8).reshape(M, N, -1)
+        a2, b2, sa2, sb2 = a.copy(), b.copy(), sa.copy(), sb.copy()
+        a2[M - 1, K - 1], b2[N // 2, 0] = 0xFF, 0x7E
+        nan = np.float32(np.nan) if scale == capi.SCALE_F32 else 255
+        sa2[1, 1], sb2[-1, -1] = nan, nan
+        got = run(a2, sa2, args[0], b2, sb2, capi.E5M2, *args[1:])
+        touched = np.zeros((M, N), bool)
+        touched[[M - 1, 1]] = True
+        touched[:, N // 2] = True
+        touched[:, (sb.shape[1] - 1) * b_rows:] = True
+        assert np.all(np.isnan(ref.from_type(got, kind)[touched]))
+        assert np.array_equal(got.view(np.uint8).reshape(M, N, -1)[~touched], clean[~touched])
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("scale,b_rows", KINDS_OF_SCALE)
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: ref.TYPE_NAMES[k])
+def test_infinity_by_every_kernel(forced, variant, scale, b_rows, kind):
+    """An e5m2 infinity gives infinities by the signs of what it meets, NaN where that is zero, in its own row alone."""
+    forced(variant)
+    for M, N, K in ((5, 40, 272), (300, 530, 400)):
+        a, sa = real_operand(M, K, capi.E5M2, scale, 1, 43)
+        b, sb = real_operand(N, K, capi.E4M3, scale, b_rows, 44)
+        b[::3, 131] = 0
+        clean = run(a, sa, capi.E5M2, b, sb, capi.E4M3, b_rows, kind).view(np.uint8).reshape(M, N, -1)
+        a[2, 131], a[4, 0] = 0x7C, 0xFC
+        got = run(a, sa, capi.E5M2, b, sb, capi.E4M3, b_rows, kind)
+        w = ref.dequantize(b, capi.E4M3, sb, b_rows)
+        for row, k, sign in ((2, 131, 1.0), (4, 0, -1.0)):
+            with np.errstate(invalid="ignore"):
+                want = sign * np.inf * w[:, k]
+            assert np.array_equal(ref.from_type(got, kind)[row], want, equal_nan=True), row
+        others = [m for m in range(M) if m not in (2, 4)]
+        assert np.array_equal(got.view(np.uint8).reshape(M, N, -1)[others], clean[others])
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("b_rows", [1, 128])
+@pytest.mark.parametrize("kind", [capi.F32, capi.BF16], ids=lambda k: ref.TYPE_NAMES[k])
+def test_every_power_of_two_as_a_scale(forced, variant, b_rows, kind):
+    """Rows scaled by each of the 255 bytes against columns scaled from the other end: every result whose two exponents add up to
+    at most 2^100 either way, among blocks whose exponents differ, is right; the rest may leave fp32 but stays by itself."""
+    forced(variant)
+    M, N, K = 255, 6 * 128, 272
+    a, b = real_operand(M, K, capi.E4M3, capi.SCALE_E8M0, 1, 45)[0], real_operand(N, K, capi.E4M3, capi.SCALE_E8M0, 1, 46)[0]
+    columns = np.array([254, 253, 190, 127, 1, 0], np.uint8)
+    sa = np.repeat(np.arange(255, dtype=np.uint8)[None], 3, 0)
+    sa[1], sa[2] = np.maximum(sa[0], 1) - 1, np.minimum(sa[0] + 1, 254)
+    sb = np.repeat((columns if b_rows == 128 else np.repeat(columns, 128))[None], 3, 0)
+    got = ref.from_type(run(a, sa, capi.E4M3, b, sb, capi.E4M3, b_rows, kind), kind)
+    power = sa[0].astype(int)[:, None] + np.repeat(columns.astype(int), 128)[None] - 254
+    x, w = ref.dequantize(a, capi.E4M3, sa, 1), ref.dequantize(b, capi.E4M3, sb, b_rows)
+    want, size = x @ w.T, np.abs(x) @ np.abs(w).T
+    largest = lambda v: np.abs(v).reshape(v.shape[0], -1, 8).max(2)  # noqa: E731
+    lost = 7 * 2.0 ** -13 * (largest(x) @ largest(w).T) if kind != capi.F32 else 0.0
+    bound = lost + size * (128 + 3 * 3 + 2) * 2.0 ** -23 + np.abs(want) * ref.HALF_STEP[kind] * 1.001        # as in check()
+    inside = np.abs(power) <= 100
+    assert inside.sum() > M * N / 3
+    bad = inside & ~(np.abs(got - want) <= bound)
+    assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5])
