@@ -502,7 +502,7 @@ int decx_hip_init(int* device) {
         HIP_TRY(hipStreamCreateWithFlags(&g_rt.stream, hipStreamNonBlocking));
         HIP_TRY(hipEventCreate(&g_rt.ev_start));
         HIP_TRY(hipEventCreate(&g_rt.ev_stop));
-        if (const char* gm = getenv("DECX_HIP_GROUP_M")) { int v = atoi(gm); if (v > 0) g_rt.group_m = v; }
+        g_rt.ask_group_m(getenv("DECX_HIP_GROUP_M"));
         if (const char* sw = getenv("DECX_HIP_SPIN_WAIT_US")) { int v = atoi(sw); if (v >= 0) g_rt.spin_wait_us = v; }
         {
             void* flag = nullptr;                              // the word the completion kernel writes and wait_compute polls

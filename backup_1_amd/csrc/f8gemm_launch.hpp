@@ -25,7 +25,7 @@ static int launch_f8gemm_tile(F8GemmArgs g) {
     const long total = (long)g.tiles_m * g.tiles_n;
     if (total * S::NT > kMostThreads) return fail(DECX_HIP_FAIL_ERROR_PARAMS, "problem too large for one launch\n");
     // raster groups 6 tile rows tall: an XCD's 32 tiles then share the fewest panels (8192^3: 400 us; 8 rows 415, 4 407, 12 413)
-    const int group_m = g_rt.group_m == Runtime().group_m ? 6 : g_rt.group_m;
+    const int group_m = g_rt.group_m_or(6);
     g.group_m = g.tiles_m < group_m ? g.tiles_m : group_m;
     hipLaunchKernelGGL(kern, dim3((unsigned)total), dim3(S::NT), S::LDS_BYTES, g_rt.stream, g);
     HIP_TRY(hipGetLastError());

@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 #include <cstddef>
 #include <cstdint>
+#include <cstdlib>
 
 #include "operands.hpp"
 
@@ -32,6 +33,12 @@ struct Runtime {
     unsigned* done_flag = nullptr; // pinned, host-coherent word a one-lane kernel behind the work stores done_seq to
     unsigned done_seq = 0;
     int group_m = 8;   // tile-rows per raster group of the XCD-aware tile walk (env DECX_HIP_GROUP_M overrides, for tuning)
+    bool group_m_asked = false;    // the environment gave it: also for kernels with a number of their own
+    void ask_group_m(const char* text) {
+        const int v = text ? atoi(text) : 0;
+        if (v > 0) group_m = v, group_m_asked = true;
+    }
+    int group_m_or(int own) const { return group_m_asked ? group_m : own; }
 };
 extern Runtime g_rt;
 
