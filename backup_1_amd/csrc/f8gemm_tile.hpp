@@ -356,6 +356,7 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
                 }
                 *reinterpret_cast<u32x2*>(park + row * ROW_BYTES + (((col >> 3) ^ (row & 7)) << 4) + ((lg & 1) << 3)) = r;
             }
+        asm volatile("" ::: "memory");                          // in this order: the lanes exchange what they hold
         uint16_t* const d = static_cast<uint16_t*>(g.D);
         const bool whole = bm0 + S::BM <= g.M && bn0 + S::BN <= g.N && ((reinterpret_cast<uintptr_t>(d) | (g.ldd * 2)) & 15) == 0;
 #pragma unroll 4
