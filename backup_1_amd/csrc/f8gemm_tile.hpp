@@ -257,7 +257,7 @@ __global__ __launch_bounds__(S::NT, 2) void f8gemm_tile_kernel(const F8GemmArgs 
     auto k_step = [&](auto stage_tag, auto ragged_tag) {
         constexpr int STG = decltype(stage_tag)::value;
         typedef std::integral_constant<int, 1 - STG> Next;
-        u32x4 keep_lo, keep_hi;
+        u32x4 keep_lo = {}, keep_hi = {};
         if constexpr (decltype(ragged_tag)::value) {
             keep_lo = unit_mask(16 * lg), keep_hi = unit_mask(16 * lg + 64);
 #pragma unroll
