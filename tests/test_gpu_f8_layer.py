@@ -234,3 +234,32 @@ def test_sizes_beyond_a_launch_are_refused(gpu):
     assert L.decx_hip_f8gemm(d.ptr, 16, 0, d.ptr, most, d.ptr, 16, 0, d.ptr, most, 128, 0, None, 0, d.ptr, most, 0, most, most, 16) == 0x0d
     assert L.decx_hip_rmsnorm_f8(d.ptr, 4096, None, 0, d.ptr, 1e-5, 0, most, 4096, d.ptr, 4096, None, None, 0, None, 0, None, 0, 0, 0) == 0x0d
     assert L.decx_hip_rmsnorm_backward(d.ptr, 64, d.ptr, d.ptr, d.ptr, 64, None, 0, 0, most + 1, 64, d.ptr, 64, None, None, 0) == 0x0d
+
+
+@pytest.mark.parametrize("M,K,F,kind,scale", [(40, 256, 384, capi.F32, capi.SCALE_F32), (200, 320, 576, capi.BF16, capi.SCALE_E8M0), (8, 136, 264, capi.F16, capi.SCALE_F32)])
+def test_training_step_operator_by_operator(gpu, M, K, F, kind, scale):
+    """What test_training_step bounds as a whole only by what 8-bit rounding costs: here each operator between the products, on what
+    the step before it made -- codes, scales and the activation bit for bit, the norm and its gradient within their own bounds."""
+    from test_gpu_rmsnorm import check, check_backward
+    s = Layer(M, K, F, kind, scale)
+    s.run()
+    capi.sync()
+    s.relu_backward()
+    s.run_rest()
+    capi.sync()
+    got = lambda n: s.d[n].result()  # noqa: E731
+    e4, e5, f32 = capi.E4M3, capi.E5M2, capi.F32
+    act, dpre = got("act"), got("dpre")
+    a = got("a")
+    assert np.array_equal(act, np.where(np.signbit(a), a * 0, a)) and np.array_equal(dpre, np.where(np.signbit(a), got("da") * 0, got("da")))
+    for name, of, of_kind, fmt, block_rows in (("qw1", s.w1, f32, e4, 128), ("qw2", s.w2, f32, e4, 128), ("qact", act, f32, e4, 1), ("qg", s.g, f32, e5, 1),
+                                               ("qd", dpre, f32, e5, 1), ("qy", got("y"), kind, e4, 1)):
+        v = ref.from_type(of, of_kind).astype(np.float32)
+        for n, m in ((name, v), (name + "t", v.T)):
+            if n == "qy":
+                continue                                         # of y before its rounding: with the norm below
+            codes, scales = ref.quantize(m, fmt, scale, block_rows)
+            values = lambda c: ref.TABLE[fmt][c]  # noqa: E731
+            assert np.array_equal(values(got(n)), values(codes)) and np.array_equal(got("s_" + n), scales), n
+    check(s.x, s.r, s.w, kind, {"H": got("h"), "rstd": got("rstd"), "Y": got("y"), "Q": got("qy"), "S": got("s_qy")}, e4, scale)
+    check_backward(got("h"), s.w, got("rstd")[0], got("dyw"), None, kind, (got("dx"), got("dw")[0]), M)
