@@ -17,7 +17,8 @@ namespace decx_hip {
 //   5: 0.64 a block of K while a CU has one tile, 1 for two; exact sums 1.15 and 2.2
 //   6: 1.05 a block of K on a nearly empty chip to 1.47 on a full one
 //   plus 2.4 (1 - 4), 3 and half of the store (5) and 7 to 11 (6) for the launch, the first loads and the store.
-// On 74 shapes from 1 x 4096 x 4096 to 4096^3, bf16 and fp32 results: within 5 % of the best kernel on all but three.
+// On 74 shapes from 1 x 4096 x 4096 to 4096^3, bf16 and fp32 results: within 5 % of the best kernel on all but three, 9 to 14 %
+// on those (profiles/f8gemm_choice_sweep.txt has every kernel's time).
 static int plan_f8gemm(int M, int N, int K, int type, int scale_type, int b_block_rows, bool aligned, bool large) {
     const int forced = g_rt.f8gemm_variant;
     if ((forced >= 1 && forced <= 4) || (forced == 5 && aligned) || (forced == 6 && aligned && large)) return forced;

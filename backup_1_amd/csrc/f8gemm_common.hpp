@@ -16,11 +16,13 @@
 //
 // What the 8-bit instructions lose.  They align the products of 8 consecutive codes to the largest of them and drop what
 // lies below 2^-13 of it (measured: 2^16 + 2^3 within 8 codes is exact, 2^16 + 2^2 gives 2^16; between groups of 8 and to
-// the accumulator nothing is dropped; v_mfma_f32_16x16x32_fp8_fp8 does the same).  On activations with outlier channels
-// that is 1e-5 to 9e-5 of the result's norm: a fifth of what rounding to binary16 costs, and less for bfloat16, but it would
-// be the whole error of an fp32 result.  Results in fp32 are therefore computed EXACTly: the codes, which binary16 holds
-// exactly in both formats, are converted in registers and multiplied by v_mfma_f32_16x16x32_f16, whose products are exact
-// and whose sums are fp32 ones (7e-8), at half the rate.
+// the accumulator nothing is dropped; v_mfma_f32_16x16x32_fp8_fp8 does the same).  A result is off by at most 7 * 2^-13 of
+// the largest product of each group of 8, added over the groups.  That is no bound relative to the result, whose sum may
+// cancel; measured as a norm, on activations with outlier channels, it is 1e-5 to 9e-5 of the result's: a fifth of what
+// rounding to binary16 costs, and less for bfloat16, but it would be the whole error of an fp32 result.  16-bit results take
+// it for twice the rate.  Results in fp32 are computed EXACTly: the codes, which binary16 holds exactly in both formats, are
+// converted in registers and multiplied by v_mfma_f32_16x16x32_f16, whose products are exact and whose sums are fp32 ones
+// (7e-8), at half the rate.
 // Accumulation is in fp32 throughout; a result is rounded to its type once.
 #pragma once
 #include "runtime.hpp"

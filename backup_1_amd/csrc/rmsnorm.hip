@@ -6,8 +6,8 @@
 //
 // Bound: memory, every element read and written once.  A workgroup owns a row at a time and keeps it in registers between
 // the sum over the row and what needs that sum; thread t holds the 8-element chunks t, t + NT, ..., so that 16 consecutive
-// lanes hold a scale block.  Sums are in fp32: at most 32 products in a thread, then a tree over lanes and waves in a fixed
-// order, which gives the same bits on every run.
+// lanes hold a scale block.  Sums are in fp32 (of rows whose squares leave its range in 64 bits): at most 32 products in a
+// thread, then a tree over lanes and waves in a fixed order, which gives the same bits on every run.
 #include "runtime.hpp"
 #include "f8_common.hpp"
 
